@@ -117,8 +117,8 @@ __global__ void k_bn_stats_final(const float* __restrict__ partial, int nblk, co
     invstd = (float)(1.0 / sqrt(var + (double)eps));
     if (running_mean) {
       const double unbiased = n > 1 ? var * ((double)n / (double)(n - 1)) : var;
-      running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * mean;
-      running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
+      running_mean[c] = mix(1.f - momentum, running_mean[c], momentum, mean);
+      running_var[c] = mix(1.f - momentum, running_var[c], momentum, (float)unbiased);
     }
   } else {
     if (!writer) return;
@@ -171,8 +171,8 @@ __global__ void k_bn_stats_final_blocks(const float* __restrict__ blocks /*[nblk
   const float invstd = (float)(1.0 / sqrt(var + (double)eps));
   if (running_mean) {
     const double unbiased = n > 1 ? var * ((double)n / (double)(n - 1)) : var;
-    running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * mean;
-    running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
+    running_mean[c] = mix(1.f - momentum, running_mean[c], momentum, mean);
+    running_var[c] = mix(1.f - momentum, running_var[c], momentum, (float)unbiased);
   }
   if (save_mean) {
     save_mean[c] = mean;

@@ -209,8 +209,8 @@ __device__ __forceinline__ void bn_fwd_fold_tile(const BnFwdFold& f, const float
   const float invstd = (float)(1.0 / sqrt(var + (double)f.eps));
   if (f.running_mean) {
     const double unbiased = n > 1 ? var * ((double)n / (double)(n - 1)) : var;
-    f.running_mean[c] = (1.f - f.momentum) * f.running_mean[c] + f.momentum * mean;
-    f.running_var[c] = (1.f - f.momentum) * f.running_var[c] + f.momentum * (float)unbiased;
+    f.running_mean[c] = mix(1.f - f.momentum, f.running_mean[c], f.momentum, mean);
+    f.running_var[c] = mix(1.f - f.momentum, f.running_var[c], f.momentum, (float)unbiased);
   }
   f.save_mean[c] = mean;
   f.save_invstd[c] = invstd;

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kCtxThreads) k_ctx_scores(const float* __restr
   for (int k = 0; k <= neg; ++k) {
     const int j = k == 0 ? g : (g + k) % B;
     const float4 c = on ? *reinterpret_cast<const float4*>(ctx + (int64_t)j * dim + 4 * t) : f4_zero();
-    red[k][t] = (s.x * c.x + s.y * c.y) + (s.z * c.z + s.w * c.w);
+    red[k][t] = f4_dot(s, c);
   }
   __syncthreads();
   for (int h = kCtxThreads / 2; h > 0; h >>= 1) {  // fixed tree: the same order every run

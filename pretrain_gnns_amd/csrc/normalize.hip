@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(kBlock) k_mean_l2norm_fwd(const float* __restr
         const float4 t = reinterpret_cast<const float4*>(sum + r * lds_)[c];
         v[q] = make_float4(t.x / cnt, t.y / cnt, t.z / cnt, t.w / cnt);
       }
-      acc += (v[q].x * v[q].x + v[q].y * v[q].y) + (v[q].z * v[q].z + v[q].w * v[q].w);
+      acc += f4_dot(v[q], v[q]);
     }
     const float nr = sqrtf(wave_sum(acc));
     const float inv = 1.f / fmaxf(nr, kNormEps);
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kBlock) k_mean_l2norm_bwd(const float* __restr
       const int c = lane + 64 * q;
       g[q] = c < d4 ? reinterpret_cast<const float4*>(dy + r * lddy)[c] : f4_zero();
       o[q] = c < d4 ? reinterpret_cast<const float4*>(y + r * ldy)[c] : f4_zero();
-      dot += (g[q].x * o[q].x + g[q].y * o[q].y) + (g[q].z * o[q].z + g[q].w * o[q].w);
+      dot += f4_dot(g[q], o[q]);
     }
     dot = wave_sum(dot);
     const float nr = norm[r];
