@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define PGNN_ABI_VERSION 11
+#define PGNN_ABI_VERSION 12
 /* uint32 words behind every `counter` argument below: the arrival tickets of a launch whose last block folds the others'
  * results (one top word + up to 32 group words: same-address atomics retire at ~50 ns each, see csrc/common.h).  Zero before
  * the first call, left zero by every call; one buffer per device serves all calls of a stream. */
@@ -38,6 +38,11 @@ extern "C" {
 #define PGNN_ERR_ARG 1
 #define PGNN_ERR_HIP 2
 #define PGNN_ERR_WORKSPACE 3
+
+/* element types of the entry points that take more than fp32 (x_type, w_type, type) */
+#define PGNN_F32 0
+#define PGNN_BF16 1
+#define PGNN_F16 2
 
 typedef void* pgnn_stream; /* hipStream_t */
 
@@ -214,6 +219,22 @@ int pgnn_neighbor_sum_bn_bwd(const float* x, int64_t ldx, const int32_t* out_ptr
                              const float* z, int64_t ldz, const float* gamma, const float* beta, const float* save_mean,
                              const float* save_invstd, int relu, int training, float* dgamma, float* dbeta, int64_t num_nodes,
                              int64_t dim, void* ws, size_t ws_bytes, const float** coef_out, int* fused, pgnn_stream stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Layer normalisation over the last axis (torch.nn.LayerNorm; no counterpart in the reference, whose networks know BatchNorm only),
+ * with the ReLU that follows it: per row  y = relu?((x - mean) rstd gamma + beta),  rstd = 1 / sqrt(var + eps), var the biased variance.
+ *   x, y [rows, dim] of x_type (PGNN_F32 / PGNN_BF16 / PGNN_F16) with leading dimensions in ELEMENTS, any alignment and any dim > 0;
+ *   gamma, beta [dim] of w_type = x_type or PGNN_F32, each may be NULL (1 and 0); save_mean / save_rstd [rows] fp32 for the backward, or
+ *   both NULL.  Statistics and sums are fp32, y is rounded once.  A row with a NaN or an infinity gives NaN in that row only.
+ * Backward: dx [rows, dim] of x_type, dgamma / dbeta [dim] of w_type, each may be NULL (not wanted); the ReLU's mask is recomputed from
+ * x.  dgamma / dbeta are added up in a fixed order (no atomics); rows == 0 writes zeros to them.  The workspace is needed for them only.
+ * ------------------------------------------------------------------------------------------ */
+int pgnn_layer_norm_fwd(const void* x, int64_t ldx, const void* gamma, const void* beta, float eps, int relu, void* y, int64_t ldy,
+                        float* save_mean, float* save_rstd, int64_t rows, int64_t dim, int x_type, int w_type, pgnn_stream stream);
+size_t pgnn_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+int pgnn_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* gamma, const void* beta, const float* save_mean,
+                        const float* save_rstd, int relu, void* dx, int64_t lddx, void* dgamma, void* dbeta, int64_t rows, int64_t dim,
+                        int x_type, int w_type, void* ws, size_t ws_bytes, pgnn_stream stream);
 
 /* ------------------------------------------------------------------------------------------
  * GraphSAGE update (chem/model.py:165-202, bio/model.py:183-224): aggr="mean" + F.normalize(p=2).

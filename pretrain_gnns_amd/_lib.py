@@ -48,6 +48,9 @@ PROTOTYPES = {
     "pgnn_bn_stats_fwd": (_i, [_p, _i64, _p, _p, _p, _p, _f, _f, _i, _p, _p, _p, _i64, _i64, _p, _sz, _p]),
     "pgnn_bn_bwd": (_i, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _p, _i64, _p, _p, _f, _u64, _i64, _i64, _p, _sz,
                          _p]),
+    "pgnn_layer_norm_fwd": (_i, [_p, _i64, _p, _p, _f, _i, _p, _i64, _p, _p, _i64, _i64, _i, _i, _p]),
+    "pgnn_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "pgnn_layer_norm_bwd": (_i, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _p, _i64, _p, _p, _i64, _i64, _i, _i, _p, _sz, _p]),
     "pgnn_mean_l2norm_fwd": (_i, [_p, _i64, _p, _p, _i64, _p, _i64, _i64, _p]),
     "pgnn_mean_l2norm_bwd": (_i, [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p]),
     "pgnn_linear_fwd": (_i, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _p]),
@@ -134,7 +137,7 @@ PROTOTYPES = {
     "pgnn_debug_aggregate_profile": (_i, [_p, _i64]),
 }
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 class GinLayer(ctypes.Structure):

@@ -50,7 +50,7 @@ class GINConv(torch.nn.Module):
             graph = ops.build_bio_graph(edge_index, edge_attr, x.size(0), gcn=False)
         agg = ops.BioAggregate.apply(x, self.edge_encoder.weight, self.edge_encoder.bias, graph)
         h = ops.linear(agg, self.mlp[0])
-        h = ops.batch_norm(h, self.mlp[1], relu=True)
+        h = ops.norm(h, self.mlp[1], relu=True)
         return ops.linear(h, self.mlp[3])
 
 
@@ -160,7 +160,7 @@ class GNN(torch.nn.Module):
     def forward(self, x, edge_index, edge_attr):
         graph = ops.build_bio_graph(edge_index, edge_attr, x.size(0), gcn=(self.gnn_type == "gcn"))
         if (_STACK_CALL and self.gnn_type == "gin" and self.JK == "last" and (self.drop_ratio == 0 or not self.training)
-                and not any(getattr(c.mlp[1], "pgnn_exact", False) for c in self.gnns)):
+                and not any(getattr(c.mlp[1], "pgnn_exact", False) or isinstance(c.mlp[1], torch.nn.LayerNorm) for c in self.gnns)):
             # the whole network as one library call per direction (ops.BioGINStack)
             return ops.bio_gin_stack(_embed_input(self.gnns[0], x), graph, list(self.gnns))
         h_list = [x]

@@ -175,7 +175,8 @@ class GNN(torch.nn.Module):
         # (a batch of the resident loader brings it along, built by offset-add: ops.attach_graph)
         graph = ops.build_chem_graph(edge_index, edge_attr, x.size(0), gcn=(self.gnn_type == "gcn"), reuse=True)
         exact_bn = getattr(self.batch_norms[0], "pgnn_exact", False)  # parallel.use_exact_batchnorm: per-layer path
-        fused = self.gnn_type == "gin" and type(self.gnns[0]) is GINConv and self.batch_norms[0].affine and not exact_bn
+        batch_bn = not any(isinstance(b, torch.nn.LayerNorm) for b in self.batch_norms)  # ops.use_layer_norm: per-layer path
+        fused = self.gnn_type == "gin" and type(self.gnns[0]) is GINConv and batch_bn and self.batch_norms[0].affine and not exact_bn
         # F.dropout of the reference (chem/model.py:271-275) is fused into the BatchNorm(+ReLU) pass
         drop_p = float(self.drop_ratio) if (self.training and self.drop_ratio > 0) else 0.0
         if fused and self.JK == "last" and _STACK_CALL and drop_p < 1.0:
@@ -183,7 +184,7 @@ class GNN(torch.nn.Module):
             return ops.chem_gin_stack(self, x, graph, self.x_embedding1, self.x_embedding2, self.gnns, self.batch_norms,
                                       drop_p)
         lin_kind = {GCNConv: 1, GraphSAGEConv: 2}.get(type(self.gnns[0]), 0)
-        if (lin_kind and self.JK == "last" and _STACK_CALL and drop_p < 1.0 and self.batch_norms[0].affine
+        if (lin_kind and self.JK == "last" and _STACK_CALL and drop_p < 1.0 and batch_bn and self.batch_norms[0].affine
                 and self.gnns[0].linear.bias is not None and not exact_bn):
             return ops.chem_lin_stack(self, lin_kind, x, graph, self.x_embedding1, self.x_embedding2, self.gnns,
                                       self.batch_norms, drop_p)
@@ -194,13 +195,13 @@ class GNN(torch.nn.Module):
             last = layer == self.num_layer - 1  # no ReLU after the last layer
             if drop_p >= 1.0:  # degenerate p = 1: everything is dropped; keep torch's semantics
                 h = self.gnns[layer](h_list[layer], edge_index, edge_attr, graph)
-                h = F.dropout(ops.batch_norm(h, self.batch_norms[layer], relu=not last), drop_p, training=True)
+                h = F.dropout(ops.norm(h, self.batch_norms[layer], relu=not last), drop_p, training=True)
             elif fused:  # conv + BatchNorm(+ReLU, +dropout) of a layer as one library call per direction
                 h = ops.chem_gin_layer(h_list[layer], self.gnns[layer], self.batch_norms[layer], graph, relu=not last,
                                        drop_p=drop_p)
             else:
                 h = self.gnns[layer](h_list[layer], edge_index, edge_attr, graph)
-                h = ops.batch_norm(h, self.batch_norms[layer], relu=not last, drop_p=drop_p)
+                h = ops.norm(h, self.batch_norms[layer], relu=not last, drop_p=drop_p)
             h_list.append(h)
 
         if self.JK == "concat":

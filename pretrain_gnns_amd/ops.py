@@ -768,6 +768,149 @@ def batch_norm(x, bn, relu, drop_p=0.0):
                                dropout_seed() if drop_p > 0 else 0)
 
 
+# ------------------------------------------------------------------------------------ layer norm
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PGNN_F32 / PGNN_BF16 / PGNN_F16
+
+
+class _on_device:
+    """the device of a tensor as the current one for the calls inside: a launch goes to the current device.  Free where it is the
+    current one already."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _call_workspace(nbytes, device):
+    """``_workspace``, but a captured call gets a buffer of its own from the graph's memory: two graphs captured on one stream may
+    be replayed side by side, and the pool's buffer would be shared by them"""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return _workspace(nbytes, device)
+
+
+def _last_axis_rows(t, dim):
+    """[rows, dim] view of a tensor whose trailing axes hold ``dim`` values, columns contiguous (any row stride); a copy where the
+    strides allow no view"""
+    t = t.reshape(-1, dim) if t.numel() else t.new_empty(0, dim)
+    return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
+
+
+def _layer_norm_fwd(x, gamma, beta, dim, eps, relu, keep):
+    rows2d = _last_axis_rows(x, dim)
+    rows = rows2d.size(0)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
+    mean = stats.data_ptr() if keep and rows else None
+    wt = gamma if gamma is not None else beta
+    check(load().pgnn_layer_norm_fwd(rows2d.data_ptr(), rows2d.stride(0), gamma.data_ptr() if gamma is not None else None,
+                                     beta.data_ptr() if beta is not None else None, eps, relu, y.data_ptr(), dim, mean,
+                                     mean + 4 * rows if mean else None, rows, dim, _TYPE_CODES[x.dtype],
+                                     _TYPE_CODES[wt.dtype if wt is not None else x.dtype], stream_ptr()), "pgnn_layer_norm_fwd")
+    return y, rows2d, stats
+
+
+class LayerNormReLU(Function):
+    """LayerNorm over the trailing axes (+ optional fused ReLU); csrc/layernorm.hip"""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, dim, eps, relu):
+        with _on_device(x.device):
+            y, rows2d, stats = _layer_norm_fwd(x, gamma, beta, dim, eps, relu, True)
+        ctx.save_for_backward(rows2d, gamma, beta, stats)
+        ctx.dim, ctx.relu, ctx.shape = dim, relu, x.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gamma, beta, stats = ctx.saved_tensors
+        dim, rows = ctx.dim, x.size(0)
+        with _on_device(x.device):
+            dy = _last_axis_rows(dy, dim)
+            need_x, need_g, need_b = ctx.needs_input_grad[:3]
+            dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device) if need_x else None
+            dgamma = torch.empty(gamma.shape, dtype=gamma.dtype, device=x.device) if need_g and gamma is not None else None
+            dbeta = torch.empty(beta.shape, dtype=beta.dtype, device=x.device) if need_b and beta is not None else None
+            ws = None
+            if dgamma is not None or dbeta is not None:
+                ws = _call_workspace(_ws_bytes("pgnn_layer_norm_bwd_workspace_bytes", rows, dim), x.device)
+            wt = gamma if gamma is not None else beta
+            ptr = lambda t: t.data_ptr() if t is not None else None
+            check(load().pgnn_layer_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), ptr(gamma), ptr(beta), stats.data_ptr(),
+                                             stats.data_ptr() + 4 * rows, ctx.relu, ptr(dx), dim, ptr(dgamma), ptr(dbeta), rows, dim,
+                                             _TYPE_CODES[x.dtype], _TYPE_CODES[wt.dtype if wt is not None else x.dtype], ptr(ws),
+                                             ws.numel() if ws is not None else 0, stream_ptr()), "pgnn_layer_norm_bwd")
+        return dx, dgamma, dbeta, None, None, None
+
+
+def layer_norm(x, ln, relu=False):
+    """apply a ``torch.nn.LayerNorm`` module's parameters with the HIP kernels, ``relu`` fuses max(., 0) behind it.  The rows are fp32,
+    bf16 or fp16 of any width and stride; the gains are of the rows' type or fp32 (mixed precision), or absent.  Statistics are per
+    row, so unlike ``batch_norm`` it takes a single row and couples no data-parallel ranks.  Gradients for x, weight and bias, added
+    up in a fixed order."""
+    gamma, beta = ln.weight, ln.bias
+    require_cuda(x, gamma, beta)
+    shape = tuple(ln.normalized_shape)
+    if x.dim() < len(shape) or tuple(x.shape[x.dim() - len(shape):]) != shape:
+        raise ValueError("layer_norm: expected trailing axes %s, got input size %s" % (shape, tuple(x.shape)))
+    if x.dtype not in _TYPE_CODES:
+        raise _lib.PgnnError("layer_norm: rows of fp32, bf16 or fp16, got %s" % x.dtype)
+    for t in (gamma, beta):
+        if t is None:
+            continue
+        if t.dtype not in (x.dtype, torch.float32) or t.dtype != (gamma if gamma is not None else beta).dtype:
+            raise _lib.PgnnError("layer_norm: gains of the rows' type (%s) or float32, both of one type, got %s" % (x.dtype, t.dtype))
+        if t.device != x.device:
+            raise _lib.PgnnError("layer_norm: rows on %s, gains on %s" % (x.device, t.device))
+        if not t.is_contiguous():
+            raise _lib.PgnnError("layer_norm: contiguous gains only")
+    dim = 1
+    for k in shape:
+        dim *= k
+    if dim == 0:
+        raise ValueError("layer_norm: nothing to normalise over in %s" % (shape,))
+    if torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
+        return LayerNormReLU.apply(x, gamma, beta, dim, float(ln.eps), int(bool(relu)))
+    with _on_device(x.device):
+        return _layer_norm_fwd(x, gamma, beta, dim, float(ln.eps), int(bool(relu)), False)[0]
+
+
+def norm(x, module, relu=False, drop_p=0.0):
+    """the normalisation of a network's layer: ``layer_norm`` for a ``torch.nn.LayerNorm``, else ``batch_norm``; ``drop_p`` > 0 is
+    the dropout behind it"""
+    if not isinstance(module, torch.nn.LayerNorm):
+        return batch_norm(x, module, relu, drop_p)
+    y = layer_norm(x, module, relu)
+    return torch.nn.functional.dropout(y, drop_p, training=True) if drop_p > 0 else y
+
+
+def use_layer_norm(module):
+    """replace every ``torch.nn.BatchNorm1d`` below ``module`` by a ``torch.nn.LayerNorm`` of its width, eps and gains: the networks
+    of chem.model and bio.model then normalise every node over its features.  The gains are new parameters (build the optimizers
+    afterwards); state-dict keys of weight and bias stay, those of the running statistics go."""
+    for name, child in list(module.named_children()):
+        if type(child) is torch.nn.BatchNorm1d:
+            where = dict(device=child.weight.device, dtype=child.weight.dtype) if child.affine else {}
+            new = torch.nn.LayerNorm(child.num_features, eps=child.eps, elementwise_affine=child.affine, **where)
+            if child.affine:
+                with torch.no_grad():
+                    new.weight.copy_(child.weight)
+                    new.bias.copy_(child.bias)
+            setattr(module, name, new.train(child.training))
+        else:
+            use_layer_norm(child)
+    return module
+
+
 # ------------------------------------------------------------------------------------ linear layers
 def _linear_fwd(x, w, b, relu):
     m, k = x.shape
