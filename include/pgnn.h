@@ -388,6 +388,26 @@ int pgnn_adam_step(float* const* params, const float* const* grads, const int64_
                    pgnn_stream stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Orthogonalisation of matrices by Newton-Schulz products, and the Muon step built on it (csrc/newton_schulz.hip; no counterpart in
+ * the reference, which knows Adam only).  For each of `count` matrices G [rows, cols] (host arrays of device pointers, sizes and leading
+ * dimensions in elements; any count, sizes 0 to 32768):
+ *   X = G / (|G|_F + eps), transposed while rows > cols; per step t, with (a, b, c) = coefficients[3 t .. 3 t + 2] (host, fp32):
+ *   A = X X^T, X <- a X + (b A + c A A) X;  result = X, dense [rows, cols] of the same `type` (PGNN_F32 / PGNN_BF16 / PGNN_F16), rounded once
+ * with the error of fp32 products throughout.  dst[j] may be src[j].  1 to 32 steps; coefficients under which the bound on X's singular
+ * values (they start in [0, 1]) passes 2^20 are refused.  A matrix of zeros gives zeros, one with a NaN or an infinity gives NaN throughout.
+ * The same workspace serves both calls; matrices are taken in chunks (at most 48, and 2 GiB of workspace unless one needs more).
+ * pgnn_muon_step: fp32, dense; per matrix  M <- mu M + G;  U = nesterov ? G + mu M : M;  p <- keep p - rates[j] orthogonal(U)
+ * (keep = 1 - lr weight_decay; rates: host).  No allocation, no atomics, bitwise reproducible; may be captured in a graph (rates, mu and
+ * keep are then the captured ones).
+ * ------------------------------------------------------------------------------------------ */
+size_t pgnn_newton_schulz_workspace_bytes(const int64_t* rows, const int64_t* cols, int64_t count);
+int pgnn_newton_schulz(const void* const* src, const int64_t* ld_src, void* const* dst, const int64_t* rows, const int64_t* cols, int64_t count,
+                       int type, const float* coefficients, int steps, float eps, void* ws, size_t ws_bytes, pgnn_stream stream);
+int pgnn_muon_step(float* const* params, const float* const* grads, float* const* momentum, const float* rates, const int64_t* rows,
+                   const int64_t* cols, int64_t count, float mu, int nesterov, float keep, const float* coefficients, int steps, float eps,
+                   void* ws, size_t ws_bytes, pgnn_stream stream);
+
+/* ------------------------------------------------------------------------------------------
  * Prediction head of the masking pre-training step, fused (chem/pretrain_masking.py:52-57; bio/pretrain_masking.py:45-56):
  *   pred = linear_pred(node_rep[idx]) ; loss = CrossEntropyLoss()(pred.double(), label) ; correct = #(argmax(pred) == label)
  * h [n_rows, ldh] node representations, idx [m] int64 rows to predict (must not repeat: MaskAtom samples without

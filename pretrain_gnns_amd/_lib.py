@@ -80,6 +80,9 @@ PROTOTYPES = {
     "pgnn_bio_gin_stack_bwd": (_i, [_p, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _p, _p, _p, _i64, _i64, _p, _sz, _p]),
     "pgnn_adam_max_tensors": (_i, []),
     "pgnn_adam_step": (_i, [_p, _p, _p, _p, _i64, _p, _p, _p, _f, _f, _f, _f, _f, _p]),
+    "pgnn_newton_schulz_workspace_bytes": (_sz, [_p, _p, _i64]),
+    "pgnn_newton_schulz": (_i, [_p, _p, _p, _p, _p, _i64, _i, _p, _i, _f, _p, _sz, _p]),
+    "pgnn_muon_step": (_i, [_p, _p, _p, _p, _p, _p, _i64, _f, _i, _f, _p, _i, _f, _p, _sz, _p]),
     "pgnn_masked_head_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "pgnn_masked_head_fwd": (_i, [_p, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "pgnn_masked_head_bwd": (_i, [_p, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _p, _p, _sz, _p]),

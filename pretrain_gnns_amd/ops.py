@@ -1896,3 +1896,71 @@ def chem_lin_stack(owner, kind, x_idx, graph, x_embedding1, x_embedding2, convs,
                                   x_embedding1.weight, x_embedding2.weight)
     return ChemLinStack.apply(x_idx, graph, (kind, training, _bn_meta(bns), drop_p, seed, plan, None),
                               x_embedding1.weight, x_embedding2.weight, *flat)
+
+
+# ------------------------------------------------------------------------------------ orthogonalisation
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _newton_schulz_coefficients(coefficients, steps):
+    """one (a, b, c) for all steps, or one per step -> a ctypes array of 3 * steps floats"""
+    import ctypes
+    if not 1 <= int(steps) <= 32:
+        raise ValueError("newton_schulz: 1 to 32 steps, got %r" % (steps,))
+    flat = list(coefficients)
+    if len(flat) == 3 and all(isinstance(v, (int, float)) for v in flat):
+        flat = flat * int(steps)
+    else:
+        if len(flat) != int(steps) or any(len(c) != 3 for c in flat):
+            raise ValueError("newton_schulz: coefficients are one (a, b, c), or one for each of the %d steps" % int(steps))
+        flat = [v for c in flat for v in c]
+    return (ctypes.c_float * len(flat))(*[float(v) for v in flat])
+
+
+def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7):
+    """orthogonalise matrices: ``steps`` Newton-Schulz products X <- a X + (b X X^T + c (X X^T)^2) X from X = G / (|G|_F + eps), which take
+    every singular value towards 1 and leave the singular vectors alone (csrc/newton_schulz.hip).  ``g``: a tensor [..., rows, cols] of
+    fp32, bf16 or fp16, or a list of such matrices of any sizes (one type and device): all of them share the launches.  Returns new
+    contiguous tensors of the same type, computed with the error of fp32 products whatever the type and rounded once.  No gradient flows
+    through it (it makes updates, not activations)."""
+    import ctypes
+    several = isinstance(g, (list, tuple))
+    tensors = list(g) if several else [g]
+    if not tensors:
+        return []
+    first = tensors[0]
+    require_cuda(*tensors)
+    coef = _newton_schulz_coefficients(coefficients, steps)
+    src, lds, rows, cols, dst, outs, held = [], [], [], [], [], [], []
+    for t in tensors:
+        if t.dtype not in _TYPE_CODES:
+            raise _lib.PgnnError("newton_schulz: matrices of fp32, bf16 or fp16, got %s" % t.dtype)
+        if t.dtype != first.dtype or t.device != first.device:
+            raise _lib.PgnnError("newton_schulz: the matrices of one call share type and device")
+        if t.dim() < 2:
+            raise ValueError("newton_schulz: matrices [..., rows, cols], got size %s" % (tuple(t.shape),))
+        r, c = t.shape[-2:]
+        with torch.no_grad():
+            m = t.detach().reshape(-1, r, c) if t.numel() else t.new_empty(0, r, c)
+            if m.numel() and ((c > 1 and m.stride(2) != 1) or m.stride(1) < 0):
+                m = m.contiguous()
+            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        held.append(m)  # (a copy has to outlive the call)
+        outs.append(out)
+        size = t.element_size()
+        for b in range(m.size(0)):
+            src.append(m.data_ptr() + b * m.stride(0) * size)
+            dst.append(out.data_ptr() + b * r * c * size)
+            lds.append(m.stride(1))
+            rows.append(r)
+            cols.append(c)
+    n = len(src)
+    if n:
+        lib = load()
+        R, C, L = (ctypes.c_int64 * n)(*rows), (ctypes.c_int64 * n)(*cols), (ctypes.c_int64 * n)(*lds)
+        with _on_device(first.device):
+            need = lib.pgnn_newton_schulz_workspace_bytes(R, C, n)
+            ws = _call_workspace(need, first.device)
+            check(lib.pgnn_newton_schulz((ctypes.c_void_p * n)(*src), L, (ctypes.c_void_p * n)(*dst), R, C, n, _TYPE_CODES[first.dtype], coef,
+                                         int(steps), float(eps), ws.data_ptr(), ws.numel(), stream_ptr()), "pgnn_newton_schulz")
+    return outs if several else outs[0]

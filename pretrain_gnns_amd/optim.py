@@ -1,4 +1,4 @@
-"""``Adam``: torch.optim.Adam's update for the optimizers of the reference's train loops, as ONE kernel launch.
+"""``Adam``: torch.optim.Adam's update for the optimizers of the reference's train loops, as ONE kernel launch; ``Muon`` beside it.
 
 The reference builds one ``optim.Adam`` per module (chem/pretrain_masking.py:134-136: model, linear_pred_atoms,
 linear_pred_bonds) with the same hyper-parameters and calls ``zero_grad()`` / ``step()`` on each.  ``Adam`` here has the
@@ -22,11 +22,26 @@ Limits, enforced rather than silent:
     while a round is incomplete, raises (the update of ALL handles would silently never be issued otherwise).
 """
 import ctypes
+import math
 
 import torch
 
 from . import _lib
-from .ops import check, load, stream_ptr
+from .ops import NEWTON_SCHULZ_COEFFICIENTS, _call_workspace, _newton_schulz_coefficients, _on_device, check, load, stream_ptr
+
+
+def _zero_grads(params, set_to_none):
+    for p in params:
+        if p.grad is None:
+            continue
+        if set_to_none:
+            p.grad = None
+        else:
+            if p.grad.grad_fn is not None:
+                p.grad.detach_()
+            else:
+                p.grad.requires_grad_(False)  # (a gradient that is a view -- parallel.GradBucket's -- cannot be detached in place)
+            p.grad.zero_()
 
 
 class _Core:
@@ -128,17 +143,7 @@ class Adam:
         if self._core.waiting != 0:
             raise _lib.PgnnError("pretrain_gnns_amd.optim.Adam.shared: zero_grad() with %d of %d handles not stepped -- the shared update "
                                  "has NOT been issued; every handle must call step() each round" % (self._core.waiting, self._core.handles))
-        for p in self._own:
-            if p.grad is None:
-                continue
-            if set_to_none:
-                p.grad = None
-            else:
-                if p.grad.grad_fn is not None:
-                    p.grad.detach_()
-                else:
-                    p.grad.requires_grad_(False)  # (a gradient that is a view -- parallel.GradBucket's -- cannot be detached in place)
-                p.grad.zero_()
+        _zero_grads(self._own, set_to_none)
 
     def step(self):
         core = self._core
@@ -156,3 +161,85 @@ class Adam:
     @property
     def step_count(self):
         return self._core.step_count
+
+
+class Muon:
+    """Muon for the weight matrices of a network: zero_grad() and step(), one library call for all of them.
+
+    Per matrix  M <- momentum M + G;  U = G + momentum M (nesterov) or M;  O = ops.newton_schulz(U, ns_steps, ns_coefficients, eps);
+    p <- p (1 - lr weight_decay) - lr s O  with s = sqrt(max(1, rows / cols)) (``adjust_lr_fn`` None or "original") or
+    0.2 sqrt(max(rows, cols)) ("match_rms_adamw": updates as large as Adam's).  The arguments are those of torch.optim.Muon; the products
+    carry fp32 error where that class multiplies in bf16.
+
+    It takes 2-D parameters only (contiguous fp32 on one GPU): biases, norms' gains and embedding tables belong to ``Adam``.  The
+    reference's loop body takes both in its optimizer list::
+
+        weights = [p for n, p in model.named_parameters() if p.dim() == 2 and "embedding" not in n]
+        others = [p for p in model.parameters() if all(p is not w for w in weights)]
+        optimizer_list = [Muon(weights, lr=0.02), Adam(others, lr=args.lr)]
+
+    ``state[p]["momentum_buffer"]`` is p's M (zero before the first step).  A parameter without a gradient is skipped, momentum and
+    all.  lr, momentum, nesterov and weight_decay are read from ``param_groups[0]`` at every step; a captured step keeps the captured ones.
+    """
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7,
+                 ns_steps=5, adjust_lr_fn=None):
+        self._own = list(params)
+        if not self._own:
+            raise ValueError("optimizer got an empty parameter list")
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError("Muon: adjust_lr_fn is None, \"original\" or \"match_rms_adamw\", got %r" % (adjust_lr_fn,))
+        if lr < 0 or momentum < 0 or weight_decay < 0 or eps < 0:
+            raise ValueError("Muon: lr, momentum, weight_decay and eps are not negative")
+        self._coef = _newton_schulz_coefficients(ns_coefficients, ns_steps)
+        for p in self._own:
+            if p.dim() != 2:
+                raise ValueError("Muon orthogonalises 2-D parameters only, got size %s: give the others to Adam" % (tuple(p.shape),))
+            if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous() or p.device != self._own[0].device:
+                raise _lib.PgnnError("pretrain_gnns_amd.optim.Muon: contiguous fp32 parameters on one GPU only")
+        if len({id(p) for p in self._own}) != len(self._own):
+            raise ValueError("Muon: a parameter appears twice")
+        self.ns_steps, self.eps, self.adjust_lr_fn = int(ns_steps), float(eps), adjust_lr_fn
+        offs, total = [], 0
+        for p in self._own:
+            offs.append(total)
+            total += (p.numel() + 63) // 64 * 64
+        self._flat = torch.zeros(total, dtype=torch.float32, device=self._own[0].device)
+        self.state = {p: {"momentum_buffer": self._flat[o:o + p.numel()].view(p.shape)} for p, o in zip(self._own, offs)}
+        self.param_groups = [{"params": self._own, "lr": lr, "weight_decay": weight_decay, "momentum": momentum, "nesterov": nesterov}]
+        self._table, self._table_key = None, None
+
+    def zero_grad(self, set_to_none=True):
+        _zero_grads(self._own, set_to_none)
+
+    def _scale(self, p):
+        rows, cols = p.shape
+        if self.adjust_lr_fn == "match_rms_adamw":
+            return 0.2 * math.sqrt(max(rows, cols))
+        return math.sqrt(max(1.0, rows / cols))
+
+    @torch.no_grad()
+    def step(self):
+        live = [p for p in self._own if p.grad is not None and p.numel()]
+        if not live:
+            return
+        lib = load()
+        key = tuple([p.data_ptr() for p in live] + [p.grad.data_ptr() for p in live])
+        if key != self._table_key:  # the tables are built again only when a pointer moved
+            for p in live:
+                if p.grad.dtype != torch.float32 or not p.grad.is_contiguous() or p.grad.device != p.device:
+                    raise _lib.PgnnError("pretrain_gnns_amd.optim.Muon: gradients must be contiguous fp32 on the parameter's device")
+            n = len(live)
+            pointers = lambda ts: (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])
+            rows, cols = (ctypes.c_int64 * n)(*[p.size(0) for p in live]), (ctypes.c_int64 * n)(*[p.size(1) for p in live])
+            self._table = (pointers(live), pointers([p.grad for p in live]), pointers([self.state[p]["momentum_buffer"] for p in live]), rows, cols, n,
+                           lib.pgnn_newton_schulz_workspace_bytes(rows, cols, n), [self._scale(p) for p in live])
+            self._table_key = key
+        P, G, M, rows, cols, n, need, scales = self._table
+        group = self.param_groups[0]
+        lr = float(group["lr"])
+        with _on_device(live[0].device):
+            ws = _call_workspace(need, live[0].device)
+            check(lib.pgnn_muon_step(P, G, M, (ctypes.c_float * n)(*[lr * s for s in scales]), rows, cols, n, float(group["momentum"]),
+                                     int(bool(group["nesterov"])), 1.0 - lr * float(group["weight_decay"]), self._coef, self.ns_steps, self.eps,
+                                     ws.data_ptr(), ws.numel(), stream_ptr()), "pgnn_muon_step")

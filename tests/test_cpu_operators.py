@@ -53,3 +53,65 @@ def test_use_layer_norm_replaces_every_batch_norm():
     with pytest.raises(_lib.PgnnError, match="no CPU fallback"):
         net(torch.zeros(1, 2, dtype=torch.long), torch.zeros(2, 0, dtype=torch.long), torch.zeros(0, 2, dtype=torch.long),
             torch.zeros(1, dtype=torch.long))
+
+
+def _arrays(shapes):
+    import ctypes
+    n = len(shapes)
+    return (ctypes.c_int64 * n)(*[r for r, _ in shapes]), (ctypes.c_int64 * n)(*[c for _, c in shapes]), n
+
+
+def test_newton_schulz_refusals():
+    import ctypes
+    with pytest.raises(_lib.PgnnError, match="no CPU fallback"):
+        ops.newton_schulz(torch.zeros(3, 4))
+    lib = _lib.load()
+    R, C, n = _arrays([(300, 600), (0, 7), (5, 4)])
+    need = lib.pgnn_newton_schulz_workspace_bytes(R, C, n)
+    assert need >= 4 * (300 * 640 + 2 * 600 * 320 + 2 * 300 * 320)  # X, X^T twice, A, B
+    many = _arrays([(64, 64)] * 1000)
+    assert lib.pgnn_newton_schulz_workspace_bytes(*many) < 60 * 100 * 1024  # taken in chunks
+    for bad in ([(32769, 1)], [(1, 32769)], [(-1, 4)]):
+        assert lib.pgnn_newton_schulz_workspace_bytes(*_arrays(bad)) == 0
+    P = (ctypes.c_void_p * 3)(4096, 4096, 4096)
+    L = (ctypes.c_int64 * 3)(600, 7, 4)
+
+    def call(rows=R, cols=C, count=n, src=P, dst=P, ld=L, kind=0, coef=(3.4445, -4.775, 2.0315), steps=5, eps=1e-7, ws=None, ws_bytes=0):
+        c = (ctypes.c_float * (3 * max(steps, 1)))(*(list(coef) * max(steps, 1)))
+        return lib.pgnn_newton_schulz(src, ld, dst, rows, cols, count, kind, c, steps, eps, ws, ws_bytes, None)
+
+    assert call() == 3 and call(ws=4096, ws_bytes=need - 1) == 3
+    assert call(count=0) == 0 and call(*_arrays([(0, 7)])) == 0  # nothing to do
+    assert call(kind=3) == 1 and call(steps=0) == 1 and call(steps=33) == 1
+    assert call(eps=-1.0) == 1 and call(eps=float("nan")) == 1
+    assert call(coef=(2.0, 2.0, 2.0)) == 1 and b"leaves every bound" in lib.pgnn_last_error()
+    assert call(coef=(float("inf"), 0.0, 0.0)) == 1
+    assert call(count=-1) == 1 and call(src=None) == 1 and call(dst=None) == 1 and call(rows=None) == 1
+    assert call(src=(ctypes.c_void_p * 3)(None, 4096, 4096), ws=4096, ws_bytes=need) == 1
+    assert call(ld=(ctypes.c_int64 * 3)(-1, 7, 4), ws=4096, ws_bytes=need) == 1
+    rates = (ctypes.c_float * 3)(1.0, 1.0, 1.0)
+    coef = (ctypes.c_float * 3)(1.5, -0.5, 0.0)
+
+    def muon(params=P, momentum=P, ws=None, ws_bytes=0):
+        return lib.pgnn_muon_step(params, P, momentum, rates, R, C, n, 0.95, 1, 1.0, coef, 1, 1e-7, ws, ws_bytes, None)
+
+    assert muon() == 3 and muon(momentum=None) == 1
+    assert muon(params=(ctypes.c_void_p * 3)(None, None, None), ws=4096, ws_bytes=need) == 1
+
+
+def test_newton_schulz_coefficient_lists():
+    make = ops._newton_schulz_coefficients
+    assert list(make((1.5, -0.5, 0.0), 2)) == [1.5, -0.5, 0.0] * 2
+    assert list(make([(1.5, -0.5, 0.0), (2, 0, 0)], 2)) == [1.5, -0.5, 0.0, 2, 0, 0]
+    assert list(make([(1, 2, 3), (4, 5, 6), (7, 8, 9)], 3)) == [1, 2, 3, 4, 5, 6, 7, 8, 9]
+    for bad in ([1, 2], [(1, 2, 3)] * 4, [(1, 2)] * 5):
+        with pytest.raises(ValueError, match="coefficients"):
+            make(bad, 5)
+
+
+def test_muon_takes_gpu_matrices_only():
+    from pretrain_gnns_amd import optim
+    with pytest.raises(_lib.PgnnError, match="one GPU"):
+        optim.Muon([torch.nn.Parameter(torch.zeros(3, 4))])
+    with pytest.raises(ValueError, match="2-D"):
+        optim.Muon([torch.nn.Parameter(torch.zeros(3))])
