@@ -1,6 +1,6 @@
 // Orthogonalisation of matrices by Newton-Schulz products, and the Muon step that is built on it:
 //   X_0 = G / (|G|_F + eps), transposed if it has more rows than columns (X is k x n, k <= n), then per step
-//   A = X X^T,  B = a I + b A + c A A,  X <- B X
+//   A = X X^T,  B = b A + c A A,  X <- a X + B X
 // which drives the singular values of X towards 1 and leaves its singular vectors alone.  Muon orthogonalises the momentum:
 //   M <- mu M + G,  U = G + mu M (nesterov) or M,  p <- p (1 - lr wd) - rate orthogonal(U)
 //
@@ -11,7 +11,8 @@
 // so ONE scale per matrix and step is known before a product runs: no row maxima, and no fp16 overflow for any input.
 // Both X and X^T are kept, so that all three products contract along rows of both operands (the fragments of an MFMA are 16-byte
 // pieces of rows): the epilogue turns its tile through LDS and writes it both ways.  A and B are symmetric: only the tiles on and
-// above the diagonal are computed, and written twice.  a I is part of B, so the last product needs no second operand.
+// above the diagonal are computed, and written twice.  a X is added behind the product B X, in fp32: as a I inside B it would stand in
+// the middle of each long sum and cost the small terms their last bits (4096 x 4096: 6.5e-6 of the 64-bit result instead of 3e-6).
 // All matrices of a call share each launch: 2 + 3 steps launches whatever their number.
 #include <algorithm>
 #include <cmath>
@@ -71,7 +72,7 @@ struct MuonArgs {
 };
 struct NoMuon { int unused; };  // (not empty: an empty kernel argument is dropped on the device side only)
 template <bool MUON> using Muon = typename std::conditional<MUON, MuonArgs, NoMuon>::type;
-struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps, max |a + b x^2 + c x^4| in step t
+struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps, max |b x^2 + c x^4| in step t
   float coef[kMaxSteps][3];
   float cap_x[kMaxSteps + 1], cap_b[kMaxSteps];
   int steps;
@@ -148,9 +149,9 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Muon<MUON> mu, Boun
       const float a = fabsf(bd.coef[t][0]), b = fabsf(bd.coef[t][1]), c = fabsf(bd.coef[t][2]);
       const float al = fmaxf(1.001f * u * u, 0x1p-60f);
       e[kMaxSteps + 1 + t] = plane_exponent(al);                                                       // A
-      const float be = fmaxf(fminf(1.001f * (a + al * (b + al * c)), bd.cap_b[t]), 0x1p-60f);
+      const float be = fmaxf(fminf(1.001f * al * (b + al * c), bd.cap_b[t]), 0x1p-60f);
       e[2 * (kMaxSteps + 1) + t] = plane_exponent(be);                                                 // B
-      u = fmaxf(fminf(be * u, bd.cap_x[t + 1]), 0x1p-60f);
+      u = fmaxf(fminf((a + be) * u, bd.cap_x[t + 1]), 0x1p-60f);
       e[t + 1] = plane_exponent(u);                                                                    // X
     }
   }
@@ -344,14 +345,20 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Muon<MUON> mu, in
         for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
       }
       const int64_t at = (int64_t)(r0 + r) * ld + c0 + c;
-      if constexpr (PHASE == kPoly) {  // + b A + a I, then to B's scale
+      if constexpr (PHASE >= kApply) {  // + a X, from X or X^T in this orientation (X is overwritten below by the thread that reads it)
+        const _Float16* X = reinterpret_cast<const _Float16*>(base + (turned ? l.x : xt_in));
+        const f16x8 h = *reinterpret_cast<const f16x8*>(X + at), lo = *reinterpret_cast<const f16x8*>(X + (int64_t)nr * ld + at);
+        const float fa = ldexpf(ca, PHASE == kApply ? eY - eX : -eX);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(fa, (float)h[e] + (float)lo[e], v[e]);
+      }
+      if constexpr (PHASE == kPoly) {  // + b A, then to B's scale
         const _Float16* A = reinterpret_cast<const _Float16*>(base + l.a);
         const f16x8 h = *reinterpret_cast<const f16x8*>(A + at), lo = *reinterpret_cast<const f16x8*>(A + (int64_t)k * ld + at);
         const float fa = ldexpf(cb, -eA), fs = ldexpf(1.f, eB);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           v[e] = fmaf(fa, (float)h[e] + (float)lo[e], v[e]);
-          if (c0 + c + e == r0 + r) v[e] += ca;
           v[e] *= fs;
         }
       }
@@ -423,7 +430,7 @@ int make_bounds(Bounds& bd, const float* coef, int steps, float eps) {
       if (!std::isfinite(coef[3 * t + q])) return 1;
       bd.coef[t][q] = coef[3 * t + q];
     }
-    bd.cap_b[t] = (float)(1.002 * even_max(coef[3 * t], coef[3 * t + 1], coef[3 * t + 2], u) + 1e-6);
+    bd.cap_b[t] = (float)(1.002 * even_max(0.0, coef[3 * t + 1], coef[3 * t + 2], u) + 1e-6);
     u = 1.002 * odd_max(coef[3 * t], coef[3 * t + 1], coef[3 * t + 2], u) + 1e-6;  // (rounding: far below the margin of 2^3 to fp16's range)
     if (!(u < 1048576.0)) return 1;
     bd.cap_x[t + 1] = (float)u;
