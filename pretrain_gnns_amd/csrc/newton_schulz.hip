@@ -9,9 +9,10 @@
 // matrix-core time of v_mfma_f32_16x16x4_f32, and two planes take the bytes of one fp32 matrix.  The iteration bounds its own
 // entries -- |X_ij| <= |X|_2 <= u_t, with u_0 = |G|_F / (|G|_F + eps) and u_{t+1} the maximum of |a x + b x^3 + c x^5| on [0, u_t] --
 // so ONE scale per matrix and step is known before a product runs: no row maxima, and no fp16 overflow for any input.
-// Both X and X^T are kept, so that all three products contract along rows of both operands (the fragments of an MFMA are 16-byte
-// pieces of rows): the epilogue turns its tile through LDS and writes it both ways.  A and B are symmetric: only the tiles on and
-// above the diagonal are computed, and written twice.  a X is added behind the product B X, in fp32: as a I inside B it would stand in
+// X is kept as X^T only: the product B X contracts along rows of B and of X^T (the fragments of an MFMA are 16-byte pieces of rows),
+// and X X^T contracts down the rows of X^T, whose fragments ds_read_b64_tr_b16 turns on their way out of LDS (keeping X as well
+// doubled what the last product writes and reads: ten 300 x 600 14.0 instead of 12.5 us).  A and B are symmetric: only the tiles on
+// and above the diagonal are computed, and written twice.  a X is added behind the product B X, in fp32: as a I inside B it would stand in
 // the middle of each long sum and cost the small terms their last bits (4096 x 4096: 6.5e-6 of the 64-bit result instead of 3e-6).
 // All matrices of a call share each launch: 2 + 3 steps launches whatever their number.
 #include <algorithm>
@@ -32,37 +33,48 @@ constexpr int64_t kChunkBytes = 2ll << 30;  // a call's matrices are taken in ch
 constexpr int kBK = 32;              // contraction per stage: one MFMA
 constexpr int kPad = 64;             // leading dimensions of the planes are multiples of this, zero beyond the matrix
 
-enum { kGram, kPoly, kApply, kLast };
+constexpr int kGram = 0, kPoly = 1, kApply = 2, kLast = 3;  // (not an unnamed enum: its name in a kernel differs between host and device)
+
+__host__ __device__ inline int parts_of(int64_t k, int64_t n) {
+  const int64_t p = (k * n + kNormPart - 1) / kNormPart;
+  return (int)(p < kMaxParts ? p : kMaxParts);
+}
 
 // where a matrix's planes are in its part of the workspace (bytes): the exponents and the partial sums in front, at fixed places; planes
 // of 64 k columns are multiples of 256 bytes by themselves
 constexpr int64_t kExps = 0, kParts = 512, kPlanes = kParts + kMaxParts * 8;
 static_assert(3 * (kMaxSteps + 1) * 4 <= kParts && kPlanes % 256 == 0, "");
 struct Layout {
-  int64_t ldk, ldn, x, xt0, xt1, a, b, bytes;
+  int64_t ldk, rows, xt0, xt1, a, b, bytes;  // X^T: `rows` rows, n of them and zeros up to whole stages
 };
 __host__ __device__ inline Layout layout_of(int64_t k, int64_t n) {
   Layout l;
   l.ldk = (k + kPad - 1) & ~(int64_t)(kPad - 1);
-  l.ldn = (n + kPad - 1) & ~(int64_t)(kPad - 1);
-  l.x = kPlanes;
-  l.xt0 = l.x + 4 * k * l.ldn;
-  l.xt1 = l.xt0 + 4 * n * l.ldk;
-  l.a = l.xt1 + 4 * n * l.ldk;
+  l.rows = (n + kBK - 1) & ~(int64_t)(kBK - 1);
+  l.xt0 = kPlanes;
+  l.xt1 = l.xt0 + 4 * l.rows * l.ldk;
+  l.a = l.xt1 + 4 * l.rows * l.ldk;
   l.b = l.a + 4 * k * l.ldk;
   l.bytes = l.b + 4 * k * l.ldk;
   return l;
 }
 
+// a matrix of the call: its first workgroup in this launch, its sizes (k <= n), whether G has more rows than columns, its workspace
+struct Job {
+  int first, k, n, tall;
+  int64_t off;
+};
 struct Jobs {
-  int count;
-  int first[kMaxJobs + 1];  // first workgroup of a job
-  int rows[kMaxJobs], cols[kMaxJobs];
-  int64_t off[kMaxJobs];    // its part of the workspace
+  int count, blocks, xcds;
+  char* ws;
+  Job job[kMaxJobs];
+};
+struct Sources {
   const void* src[kMaxJobs];  // G
   int64_t ld[kMaxJobs];
-  void* dst[kMaxJobs];      // the result, or the parameter
-  char* ws;
+};
+struct Results {
+  void* dst[kMaxJobs];        // the orthogonal matrix, or the parameter
 };
 struct MuonArgs {
   float* momentum[kMaxJobs];
@@ -70,8 +82,9 @@ struct MuonArgs {
   float mu, keep;           // keep = 1 - lr wd
   int nesterov;
 };
-struct NoMuon { int unused; };  // (not empty: an empty kernel argument is dropped on the device side only)
-template <bool MUON> using Muon = typename std::conditional<MUON, MuonArgs, NoMuon>::type;
+struct Nothing { int unused; };  // (not empty: an empty kernel argument is dropped on the device side only)
+template <bool MUON> using Muon = typename std::conditional<MUON, MuonArgs, Nothing>::type;
+template <int PHASE> using Last = typename std::conditional<PHASE == kLast, Results, Nothing>::type;
 struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps, max |b x^2 + c x^4| in step t
   float coef[kMaxSteps][3];
   float cap_x[kMaxSteps + 1], cap_b[kMaxSteps];
@@ -79,57 +92,101 @@ struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps
   float eps;
 };
 
-__device__ __forceinline__ int find_job(const int* first, int count, int b) {
-  int j = 0, hi = count;
-  while (hi - j > 1) {
-    const int mid = (j + hi) >> 1;
-    if (first[mid] <= b) j = mid; else hi = mid;
-  }
-  return j;
+// the job of a workgroup, found by one vector load and a ballot: a bisection is a chain of scalar loads, each of which waits for the
+// kernel arguments anew
+__device__ __forceinline__ int find_job(const Jobs& jobs, int b) {
+  const int lane = threadIdx.x & 63;
+  const int first = lane < jobs.count ? jobs.job[lane].first : 0x7fffffff;
+  return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(first <= b)) - 1);
 }
+// 16 bytes of G at the element's own alignment
+template <typename T> struct Piece { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); static constexpr int n = 16 / sizeof(T); };
 
 // partial sums of squares in float64 (millions of terms, squares of gradients far below 1); Muon: the momentum is advanced here
 template <typename T, bool MUON>
-__global__ void __launch_bounds__(256) k_ns_norm(Jobs jobs, Muon<MUON> mu) {
-  const int j = find_job(jobs.first, jobs.count, blockIdx.x);
-  const int part = blockIdx.x - jobs.first[j], nparts = jobs.first[j + 1] - jobs.first[j];
-  const int64_t rows = jobs.rows[j], cols = jobs.cols[j];
+__global__ void __launch_bounds__(256) k_ns_norm(Jobs jobs, Sources from, Muon<MUON> mu) {
+  const int j = find_job(jobs, blockIdx.x);
+  const Job job = jobs.job[j];
+  const int rows = job.tall ? job.n : job.k, cols = job.tall ? job.k : job.n;
+  const int nparts = parts_of(job.k, job.n), part = blockIdx.x - job.first;
+  const T* g = static_cast<const T*>(from.src[j]);
+  const int64_t ld = from.ld[j];
+  constexpr int E = Piece<T>::n;
   double s = 0.0;
-  const int64_t stride = (int64_t)nparts * 256;
-  for (int64_t e = (int64_t)part * 256 + threadIdx.x; e < rows * cols; e += stride) {
-    const int64_t r = e / cols, c = e - r * cols;
-    float v = (float)static_cast<const T*>(jobs.src[j])[r * jobs.ld[j] + c];
+  auto add = [&](float v, float& m) {
     if constexpr (MUON) {
-      const float m = fmaf(mu.mu, mu.momentum[j][e], v);
-      mu.momentum[j][e] = m;
+      m = fmaf(mu.mu, m, v);
       v = mu.nesterov ? fmaf(mu.mu, m, v) : m;
     }
     s += (double)v * (double)v;
+  };
+  // a dense matrix is one long row; else the workgroup's lanes walk the pieces of row after row
+  const bool dense = ld == cols || rows == 1;
+  const int64_t width = dense ? (int64_t)rows * cols : cols, pieces = (width + E - 1) / E;
+  const int64_t stride = (int64_t)nparts * 256, start = (int64_t)part * 256 + threadIdx.x;
+  int64_t r = 0, c = start;
+  if (!dense) { r = start / pieces; c = start - r * pieces; }
+  const int64_t dr = dense ? 0 : stride / pieces, dc = dense ? stride : stride - dr * pieces;
+  while (dense ? c < pieces : r < rows) {
+    const int64_t at = r * ld + c * E;
+    [[maybe_unused]] float* m = nullptr;
+    if constexpr (MUON) m = mu.momentum[j] + at;  // (dense: ld == cols)
+    if (c * E + E <= width) {
+      const typename Piece<T>::type p = *reinterpret_cast<const typename Piece<T>::type*>(g + at);
+      typename Piece<float>::type mv = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (MUON) mv = *reinterpret_cast<typename Piece<float>::type*>(m);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float t = mv[e & 3];
+        add((float)p[e], t);
+        mv[e & 3] = t;
+      }
+      if constexpr (MUON) *reinterpret_cast<typename Piece<float>::type*>(m) = mv;
+    } else {
+      for (int e = 0; e < E && c * E + e < width; ++e) {
+        float t = 0.f;
+        if constexpr (MUON) t = m[e];
+        add((float)g[at + e], t);
+        if constexpr (MUON) m[e] = t;
+      }
+    }
+    c += dc;
+    r += dr;
+    if (!dense && c >= pieces) { c -= pieces; ++r; }
   }
   __shared__ double lds[4];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    reinterpret_cast<double*>(jobs.ws + jobs.off[j] + kParts)[part] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
-  }
+  if (threadIdx.x == 0)
+    reinterpret_cast<double*>(jobs.ws + job.off + kParts)[part] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
 // exponent e with bound * 2^e <= 2^13 (entries then stay a factor of 8 below fp16's largest value)
 __device__ __forceinline__ int plane_exponent(float bound) { return 12 - ilogbf(bound); }
 
-// X_0 as planes, both ways round, and the exponents of all planes to come
+__device__ __forceinline__ void split8(const float (&v)[8], f16x8& h, f16x8& l) {
+  uint32_t hh[4], ll[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) split2(v[2 * q], v[2 * q + 1], hh[q], ll[q]);
+  h = __builtin_bit_cast(f16x8, make_uint4(hh[0], hh[1], hh[2], hh[3]));
+  l = __builtin_bit_cast(f16x8, make_uint4(ll[0], ll[1], ll[2], ll[3]));
+}
+
+// X_0^T as planes, and the exponents of all planes to come
 template <typename T, bool MUON>
-__global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Muon<MUON> mu, Bounds bd) {
-  const int j = find_job(jobs.first, jobs.count, blockIdx.x);
-  const int64_t rows = jobs.rows[j], cols = jobs.cols[j];
-  const bool tall = rows > cols;
-  const Layout l = layout_of(min(rows, cols), max(rows, cols));
-  char* base = jobs.ws + jobs.off[j];
+__global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<MUON> mu, Bounds bd) {
+  const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
+  const int j = find_job(jobs, b);
+  const Job job = jobs.job[j];
+  const bool tall = job.tall;
+  const int rows = tall ? job.n : job.k, cols = tall ? job.k : job.n;
+  const Layout l = layout_of(job.k, job.n);
+  char* base = jobs.ws + job.off;
   __shared__ float tile[64][65];
   __shared__ double red[4];
-  const int nparts = (int)min((int64_t)kMaxParts, (rows * cols + kNormPart - 1) / kNormPart);
+  const int nparts = parts_of(job.k, job.n);
   double s = (int)threadIdx.x < nparts ? reinterpret_cast<const double*>(base + kParts)[threadIdx.x] : 0.0;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
@@ -141,7 +198,7 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Muon<MUON> mu, Boun
   if (!(u >= 0x1p-60f)) u = 0x1p-60f;  // (also a NaN: everything becomes NaN whatever the scale)
   if (!(u <= bd.cap_x[0])) u = bd.cap_x[0];
   const int e0 = plane_exponent(u);
-  const int local = blockIdx.x - jobs.first[j];
+  const int local = b - job.first;
   if (local == 0 && threadIdx.x == 0) {
     int* e = reinterpret_cast<int*>(base + kExps);
     e[0] = e0;
@@ -157,126 +214,220 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Muon<MUON> mu, Boun
   }
   const int tc = (int)((cols + 63) / 64), r0 = local / tc * 64, c0 = local % tc * 64;
   const float scale = ldexpf(1.f, e0);
-  for (int q = threadIdx.x; q < 4096; q += 256) {
-    const int r = q >> 6, c = q & 63;
-    float v = 0.f;
-    if (r0 + r < rows && c0 + c < cols) {
-      v = (float)static_cast<const T*>(jobs.src[j])[(r0 + r) * jobs.ld[j] + c0 + c];
-      if constexpr (MUON) {  // the direction, from the momentum that k_ns_norm has advanced
-        const float m = mu.momentum[j][(r0 + r) * cols + c0 + c];
-        v = mu.nesterov ? fmaf(mu.mu, m, v) : m;
+  const T* g = static_cast<const T*>(from.src[j]);
+  const int64_t ld = from.ld[j];
+  constexpr int E = Piece<T>::n, ACROSS = 64 / E;
+#pragma unroll
+  for (int q = 0; q < 64 * ACROSS / 256; ++q) {
+    const int i = q * 256 + threadIdx.x, r = i / ACROSS, c = i % ACROSS * E;
+    float v[E];
+    const bool in = r0 + r < rows;
+    if (in && c0 + c + E <= cols) {
+      const typename Piece<T>::type p = *reinterpret_cast<const typename Piece<T>::type*>(g + (r0 + r) * ld + c0 + c);
+      typename Piece<float>::type m = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (MUON) m = *reinterpret_cast<const typename Piece<float>::type*>(mu.momentum[j] + (int64_t)(r0 + r) * cols + c0 + c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[e] = (float)p[e];
+        if constexpr (MUON) v[e] = mu.nesterov ? fmaf(mu.mu, m[e & 3], v[e]) : m[e & 3];  // the momentum that k_ns_norm has advanced
       }
-      v = v * inv * scale;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[e] = 0.f;
+        if (in && c0 + c + e < cols) {
+          v[e] = (float)g[(r0 + r) * ld + c0 + c + e];
+          if constexpr (MUON) {
+            const float m = mu.momentum[j][(int64_t)(r0 + r) * cols + c0 + c + e];
+            v[e] = mu.nesterov ? fmaf(mu.mu, m, v[e]) : m;
+          }
+        }
+      }
     }
-    tile[r][c] = v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) tile[r][c + e] = v[e] * inv * scale;
   }
   __syncthreads();
-  _Float16* as_is = reinterpret_cast<_Float16*>(base + (tall ? l.xt0 : l.x));
-  _Float16* turned = reinterpret_cast<_Float16*>(base + (tall ? l.x : l.xt0));
-  const int64_t ld_is = tall ? l.ldk : l.ldn, ld_tu = tall ? l.ldn : l.ldk;
+  _Float16* d = reinterpret_cast<_Float16*>(base + l.xt0);
+  const int dr0 = tall ? r0 : c0, dc0 = tall ? c0 : r0;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    _Float16* d = half ? turned : as_is;
-    const int64_t ld = half ? ld_tu : ld_is, dr0 = half ? c0 : r0, dc0 = half ? r0 : c0, drows = half ? cols : rows;
-    for (int q = threadIdx.x; q < 64 * 32; q += 256) {
-      const int r = q >> 5, c = (q & 31) * 2;
-      if (dr0 + r >= drows) continue;
-      uint32_t h, lo;
-      split2(half ? tile[c][r] : tile[r][c], half ? tile[c + 1][r] : tile[r][c + 1], h, lo);
-      *reinterpret_cast<uint32_t*>(d + (dr0 + r) * ld + dc0 + c) = h;
-      *reinterpret_cast<uint32_t*>(d + (drows + dr0 + r) * ld + dc0 + c) = lo;
+  for (int q = 0; q < 2; ++q) {
+    const int i = q * 256 + threadIdx.x, r = i >> 3, c = (i & 7) * 8;
+    if (dr0 + r >= (int)l.rows) continue;  // (rows n .. l.rows: zeros)
+    float v[8];
+    if (tall) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
     }
+    f16x8 h, lo;
+    split8(v, h, lo);
+    const int64_t at = (int64_t)(dr0 + r) * l.ldk + dc0 + c;
+    *reinterpret_cast<f16x8*>(d + at) = h;
+    *reinterpret_cast<f16x8*>(d + l.rows * l.ldk + at) = lo;
   }
 }
 
+// tile (ti, tj) of a launch's local index: columns of tiles in bands of kBand, a band row by row, so that the workgroups that run at the
+// same time on an XCD (it takes a contiguous range) share kBand rows and columns of tiles in its L2.  symmetric: ti <= tj only
+constexpr int kBand = 8;
 template <typename T> struct Out8 { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
-
-__device__ __forceinline__ void split8(const float (&v)[8], f16x8& h, f16x8& l) {
-  uint32_t hh[4], ll[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) split2(v[2 * q], v[2 * q + 1], hh[q], ll[q]);
-  h = __builtin_bit_cast(f16x8, make_uint4(hh[0], hh[1], hh[2], hh[3]));
-  l = __builtin_bit_cast(f16x8, make_uint4(ll[0], ll[1], ll[2], ll[3]));
+__device__ __forceinline__ void tile_at(int local, int down, int across, bool symmetric, int& ti, int& tj) {
+  if (!symmetric) {
+    const int band = local / (down * kBand), rem = local - band * down * kBand, w = min(kBand, across - band * kBand);
+    ti = rem / w;
+    tj = band * kBand + rem - ti * w;
+    return;
+  }
+  // full bands before band b hold kBand^2 b (b - 1) / 2 + b kBand (kBand + 1) / 2 = 32 b^2 + 4 b tiles
+  int band = (int)((sqrtf(16.f + 128.f * (float)local) - 4.f) * (1.f / 64.f));
+  while (32 * band * band + 4 * band > local) --band;
+  while (32 * (band + 1) * (band + 1) + 4 * (band + 1) <= local) ++band;
+  const int rem = local - (32 * band * band + 4 * band), first = band * kBand, w = min(kBand, across - first);
+  if (rem < first * w) {
+    ti = rem / w;
+    tj = first + rem - ti * w;
+  } else {  // the triangle on the diagonal, column by column
+    int t = rem - first * w;
+    tj = first;
+    while (t > tj - first) {
+      t -= tj - first + 1;
+      ++tj;
+    }
+    ti = first + t;
+  }
 }
 
-// One TT x TT tile of C = P Q^T, P and Q on planes.  Four waves of TT/2 x TT/2; wave w fetches operand array w (P high, P low, Q high,
-// Q low) by LDS DMA, STAGES - 1 stages ahead.  A stage holds 32 columns: 64 bytes per row, whose four 16-byte pieces are permuted by
-// (row >> 1) & 3, so that the eight rows one LDS cycle reads of a piece lie in eight different bank groups.
+// four blocks of 16 columns x 32 l, both planes, turned on their way out of LDS: at[b] the lane's address of block b, H the distance of
+// l + 4, ARR that of the low plane.  One asm block with its own wait: with the builtin hipcc waits for every DMA in flight in front of the
+// reads (ten 300 x 600: X X^T 15.7 us instead of 11.0), and a load of inline asm must not leave its block unfinished.
+template <int H, int ARR>
+__device__ __forceinline__ void read_turned(const uint32_t (&at)[4], f16x8 (&hi)[4], f16x8 (&lo)[4]) {
+  uint2 r[4][4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%20\n\tds_read_b64_tr_b16 %2, %16 offset:%21\n\tds_read_b64_tr_b16 %3, %16 offset:%22\n\t"
+      "ds_read_b64_tr_b16 %4, %17\n\tds_read_b64_tr_b16 %5, %17 offset:%20\n\tds_read_b64_tr_b16 %6, %17 offset:%21\n\tds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
+      "ds_read_b64_tr_b16 %8, %18\n\tds_read_b64_tr_b16 %9, %18 offset:%20\n\tds_read_b64_tr_b16 %10, %18 offset:%21\n\tds_read_b64_tr_b16 %11, %18 offset:%22\n\t"
+      "ds_read_b64_tr_b16 %12, %19\n\tds_read_b64_tr_b16 %13, %19 offset:%20\n\tds_read_b64_tr_b16 %14, %19 offset:%21\n\tds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3]),
+        "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[2][2]), "=&v"(r[2][3]), "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[3][2]), "=&v"(r[3][3])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(H), "n"(ARR), "n"(ARR + H)
+      : "memory");
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    hi[b] = __builtin_bit_cast(f16x8, make_uint4(r[b][0].x, r[b][0].y, r[b][1].x, r[b][1].y));
+    lo[b] = __builtin_bit_cast(f16x8, make_uint4(r[b][2].x, r[b][2].y, r[b][3].x, r[b][3].y));
+  }
+}
+
+// One TT x TT tile of a product on planes, C[i][j] = sum_l P(i, l) Q(j, l).  Four waves of TT/2 x TT/2; wave w fetches operand array w
+// (P high, P low, Q high, Q low) by LDS DMA, STAGES - 1 stages ahead.  A stage is 32 deep.
+//   A A and B X: l runs along the operands' rows.  A stage holds 64 bytes of TT rows, whose four 16-byte pieces are permuted by
+//   (row >> 1) & 3, so that the eight rows of a piece that one LDS cycle reads lie in eight different bank groups.
+//   X X^T: l runs down the rows of X^T.  A stage holds 32 rows of 2 TT bytes; a fragment (8 l of one column per lane) is two
+//   ds_read_b64_tr_b16, each of which hands a 16-lane group a 4 x 16 block turned.  The 32-byte blocks of a row are permuted by bits of
+//   the row, so that the 16 rows that one instruction reads lie evenly over the banks.
 template <int TT, int STAGES, int PHASE, typename TO, bool MUON>
-__global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Muon<MUON> mu, int step, float ca, float cb, float cc) {
+__global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
   constexpr int MI = TT / 32, ARR = TT * kBK * 2, STAGE = 4 * ARR, NJ = TT / 16;
   constexpr int LDT = TT + 4;  // floats per row of the epilogue's tile: 16-byte rows, neighbours four banks apart
   extern __shared__ __align__(16) char smem[];
-  const int j = find_job(jobs.first, jobs.count, blockIdx.x);
-  const int rows = jobs.rows[j], cols = jobs.cols[j], k = min(rows, cols), n = max(rows, cols);
+  const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
+  const int j = find_job(jobs, b);
+  const Job job = jobs.job[j];
+  const int k = job.k, n = job.n;
   const Layout l = layout_of(k, n);
-  char* base = jobs.ws + jobs.off[j];
+  char* base = jobs.ws + job.off;
   int ti, tj;
-  {
-    const int local = blockIdx.x - jobs.first[j];
-    if constexpr (PHASE <= kPoly) {  // tile pairs ti <= tj, column by column
-      tj = (int)((sqrtf(8.f * (float)local + 1.f) - 1.f) * 0.5f);
-      while (tj * (tj + 1) / 2 > local) --tj;
-      while ((tj + 1) * (tj + 2) / 2 <= local) ++tj;
-      ti = local - tj * (tj + 1) / 2;
-    } else {
-      const int across = (k + TT - 1) / TT;
-      ti = local % across;
-      tj = local / across;
-    }
-  }
+  tile_at(b - job.first, (k + TT - 1) / TT, ((PHASE <= kPoly ? k : n) + TT - 1) / TT, PHASE <= kPoly, ti, tj);
   const int* exps = reinterpret_cast<const int*>(base + kExps);
   const int eX = exps[step], eA = exps[kMaxSteps + 1 + step], eB = exps[2 * (kMaxSteps + 1) + step], eY = exps[step + 1];
   const int64_t xt_in = step & 1 ? l.xt1 : l.xt0, xt_out = step & 1 ? l.xt0 : l.xt1;
-  // operands: rows, leading dimension, planes
-  const _Float16 *P, *Q;
-  int prow, qrow, ldp, kk;
-  if constexpr (PHASE == kGram) {
-    P = Q = reinterpret_cast<const _Float16*>(base + l.x);
-    prow = qrow = k;
-    ldp = kk = (int)l.ldn;
-  } else if constexpr (PHASE == kPoly) {
-    P = Q = reinterpret_cast<const _Float16*>(base + l.a);
-    prow = qrow = k;
-    ldp = kk = (int)l.ldk;
-  } else {
-    P = reinterpret_cast<const _Float16*>(base + l.b);
-    Q = reinterpret_cast<const _Float16*>(base + xt_in);
-    prow = k;
-    qrow = n;
-    ldp = kk = (int)l.ldk;
-  }
+  const _Float16* XT = reinterpret_cast<const _Float16*>(base + xt_in);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int i0 = ti * TT, j0 = tj * TT;
+  const int i0 = ti * TT, j0 = tj * TT, ldk = (int)l.ldk;
 
-  // the wave's DMA pieces: 16 rows of 64 bytes each
-  const _Float16* src = (wave < 2 ? P + (int64_t)(wave & 1) * prow * ldp : Q + (int64_t)(wave & 1) * qrow * ldp);
-  uint32_t offs[NJ];  // in halfs; rows beyond the matrix re-read its last one (their results are not stored)
+  // the wave's DMA pieces: 1 KB each
+  const _Float16* src;
+  uint32_t offs[NJ];  // in halfs; what lies beyond the matrix re-reads its last row or column (the results are not stored)
+  int64_t advance;    // per stage
+  int nk;
+  if constexpr (PHASE == kGram) {
+    constexpr int UNITS = TT / 8, ROWS = 64 / UNITS;  // 16-byte units per row, rows per piece
+    src = XT + (wave & 1) * l.rows * ldk;
+    nk = (int)l.rows / kBK;
+    advance = (int64_t)kBK * ldk;
 #pragma unroll
-  for (int q = 0; q < NJ; ++q) {
-    const int r = q * 16 + (lane >> 2);
-    const int row = min((wave < 2 ? i0 : j0) + r, (wave < 2 ? prow : qrow) - 1);
-    offs[q] = (uint32_t)row * (uint32_t)ldp + (uint32_t)(((lane & 3) ^ ((r >> 1) & 3)) * 8);
+    for (int q = 0; q < NJ; ++q) {
+      const int r = q * ROWS + lane / UNITS, u = lane % UNITS;
+      const int turn = TT == 64 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r & 3) | ((r >> 1) & 4);
+      const int col = (wave < 2 ? i0 : j0) + (((u >> 1) ^ turn) * 2 + (u & 1)) * 8;
+      offs[q] = (uint32_t)r * (uint32_t)ldk + (uint32_t)min(col, ldk - 8);
+    }
+  } else {
+    const _Float16* P = reinterpret_cast<const _Float16*>(base + (PHASE == kPoly ? l.a : l.b));
+    const _Float16* Q = PHASE == kPoly ? P : XT;
+    const int qrows = PHASE == kPoly ? k : (int)l.rows;
+    src = wave < 2 ? P + (int64_t)(wave & 1) * k * ldk : Q + (int64_t)(wave & 1) * qrows * ldk;
+    nk = ldk / kBK;
+    advance = kBK;
+#pragma unroll
+    for (int q = 0; q < NJ; ++q) {
+      const int r = q * 16 + (lane >> 2);
+      const int row = min((wave < 2 ? i0 : j0) + r, (wave < 2 ? k : qrows) - 1);
+      offs[q] = (uint32_t)row * (uint32_t)ldk + (uint32_t)(((lane & 3) ^ ((r >> 1) & 3)) * 8);
+    }
   }
   auto issue = [&](int t) {
     char* dst = smem + (t % STAGES) * STAGE + wave * ARR;
 #pragma unroll
     for (int q = 0; q < NJ; ++q)
-      __builtin_amdgcn_global_load_lds(PGNN_GPTR(src + (size_t)offs[q] + (size_t)t * kBK), PGNN_LPTR(dst + q * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(PGNN_GPTR(src + (size_t)offs[q] + (size_t)t * advance), PGNN_LPTR(dst + q * 1024), 16, 0, 0);
   };
+
+  // the epilogue's operand (A behind A A, X^T behind B X) at this thread's pieces of the tile, fetched in front of everything else: its
+  // round trip to memory hides behind the product
+  constexpr int PIECES = TT / 8, MINE = TT * PIECES / 256;  // 16-byte pieces per row, pieces per thread
+  const int out_rows = PHASE <= kPoly ? k : (int)l.rows;
+  [[maybe_unused]] f16x8 eh[MINE], el[MINE];
+  if constexpr (PHASE != kGram) {
+    const _Float16* E = PHASE == kPoly ? reinterpret_cast<const _Float16*>(base + l.a) : XT;
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) {
+      const int r = (q * 256 + threadIdx.x) / PIECES, c = (threadIdx.x % PIECES) * 8;
+      const int64_t at = (int64_t)min(j0 + r, out_rows - 1) * ldk + min(i0 + c, ldk - 8);
+      eh[q] = *reinterpret_cast<const f16x8*>(E + at);
+      el[q] = *reinterpret_cast<const f16x8*>(E + (int64_t)out_rows * ldk + at);
+    }
+  }
+
   const int wi = (wave >> 1) * (TT / 2), wj = (wave & 1) * (TT / 2);
   const int fr = lane & 15, fc = lane >> 4;
-  auto frag = [&](const char* arr, int row) {
-    return *reinterpret_cast<const f16x8*>(arr + row * 64 + ((fc ^ ((row >> 1) & 3)) * 16));
-  };
+  // byte offsets of the lane's fragments inside a stage: block a of the wave's rows i and of its rows j (X X^T: of its columns)
+  uint32_t pat[MI], qat[MI];
+#pragma unroll
+  for (int a = 0; a < MI; ++a) {
+    const int pb = wi / 16 + a, qb = wj / 16 + a;
+    if constexpr (PHASE == kGram) {  // rows l = 8 fc + fr / 4; the rows l + 4 have the same permutation
+      const int r = 8 * fc + (fr >> 2);
+      const int turn = TT == 64 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r & 3) | ((r >> 1) & 4);
+      pat[a] = (uint32_t)(r * TT * 2 + (pb ^ turn) * 32 + (fr & 3) * 8);
+      qat[a] = (uint32_t)(r * TT * 2 + (qb ^ turn) * 32 + (fr & 3) * 8 + 2 * ARR);
+    } else {
+      pat[a] = (uint32_t)((pb * 16 + fr) * 64 + ((fc ^ ((fr >> 1) & 3)) * 16));
+      qat[a] = (uint32_t)((qb * 16 + fr) * 64 + ((fc ^ ((fr >> 1) & 3)) * 16) + 2 * ARR);
+    }
+  }
 
   f32x4 acc[MI][MI];
 #pragma unroll
   for (int a = 0; a < MI; ++a)
 #pragma unroll
-    for (int b = 0; b < MI; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < MI; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int nk = kk / kBK;
 #pragma unroll
   for (int t = 0; t < STAGES - 1; ++t)
     if (t < nk) issue(t);
@@ -290,105 +441,126 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Muon<MUON> mu, in
     if (t + STAGES - 1 < nk) issue(t + STAGES - 1);
     const char* st = smem + (t % STAGES) * STAGE;
     f16x8 ph[MI], pl[MI], qh[MI], ql[MI];
+    if constexpr (PHASE == kGram) {
+      const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)st;
+      if constexpr (MI == 2) {
+        f16x8 h[4], lo[4];
+        read_turned<4 * TT * 2, ARR>({at + pat[0], at + pat[1], at + qat[0], at + qat[1]}, h, lo);
 #pragma unroll
-    for (int a = 0; a < MI; ++a) {
-      ph[a] = frag(st, wi + a * 16 + fr);
-      pl[a] = frag(st + ARR, wi + a * 16 + fr);
-      qh[a] = frag(st + 2 * ARR, wj + a * 16 + fr);
-      ql[a] = frag(st + 3 * ARR, wj + a * 16 + fr);
+        for (int a = 0; a < 2; ++a) { ph[a] = h[a]; pl[a] = lo[a]; qh[a] = h[2 + a]; ql[a] = lo[2 + a]; }
+      } else {
+        static_assert(MI == 2 || MI == 4, "");
+        read_turned<4 * TT * 2, ARR>({at + pat[0], at + pat[1], at + pat[2], at + pat[3]}, ph, pl);
+        read_turned<4 * TT * 2, ARR>({at + qat[0], at + qat[1], at + qat[2], at + qat[3]}, qh, ql);
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < MI; ++a) {
+        ph[a] = *reinterpret_cast<const f16x8*>(st + pat[a]);
+        pl[a] = *reinterpret_cast<const f16x8*>(st + pat[a] + ARR);
+        qh[a] = *reinterpret_cast<const f16x8*>(st + qat[a]);
+        ql[a] = *reinterpret_cast<const f16x8*>(st + qat[a] + ARR);
+      }
     }
 #pragma unroll
-    for (int b = 0; b < MI; ++b) {  // smallest terms first
+    for (int c = 0; c < MI; ++c) {  // smallest terms first
 #pragma unroll
-      for (int a = 0; a < MI; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], ql[b], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < MI; ++a) acc[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], ql[c], acc[a][c], 0, 0, 0);
 #pragma unroll
-      for (int a = 0; a < MI; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[a], qh[b], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < MI; ++a) acc[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[a], qh[c], acc[a][c], 0, 0, 0);
 #pragma unroll
-      for (int a = 0; a < MI; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], qh[b], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < MI; ++a) acc[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], qh[c], acc[a][c], 0, 0, 0);
     }
     asm volatile("" ::: "memory");
   }
 
-  // epilogue: the tile to LDS as fp32 [j][i] (a lane holds four consecutive i of one j), then out row by row, both ways
+  // epilogue: the tile to LDS as fp32 [j][i] (a lane holds four consecutive i of one j), out row by row as the operand lies (rows j),
+  // and once more turned (rows i) where the mirror image of a symmetric tile or a wide G wants it
   __syncthreads();
   float* tile = reinterpret_cast<float*>(smem);
-  const float f = PHASE == kGram ? ldexpf(1.f, eA - 2 * eX) : PHASE == kPoly ? ldexpf(cc, -2 * eA)
+  const float f = PHASE == kGram ? ldexpf(1.f, eA - 2 * eX) : PHASE == kPoly ? ldexpf(cc, eB - 2 * eA)
                 : PHASE == kApply ? ldexpf(1.f, eY - eX - eB) : ldexpf(1.f, -eX - eB);
+  const float fe = PHASE == kPoly ? ldexpf(cb, eB - eA) : PHASE == kApply ? ldexpf(ca, eY - eX) : ldexpf(ca, -eX);
 #pragma unroll
   for (int a = 0; a < MI; ++a)
 #pragma unroll
-    for (int b = 0; b < MI; ++b)
-      *reinterpret_cast<f32x4*>(tile + (wj + b * 16 + fr) * LDT + wi + a * 16 + fc * 4) = acc[a][b] * f;
+    for (int c = 0; c < MI; ++c)
+      *reinterpret_cast<f32x4*>(tile + (wj + c * 16 + fr) * LDT + wi + a * 16 + fc * 4) = acc[a][c] * f;
   __syncthreads();
-  constexpr int PIECES = TT / 8;
-  const bool tall = rows > cols;
-#pragma unroll
-  for (int turned = 0; turned < 2; ++turned) {
-    // turned = 0: rows j of the transpose, columns i; turned = 1: rows i, columns j
+
+  auto planes_out = [&](_Float16* d, int rows, int64_t at, const float (&v)[8]) {
+    f16x8 h, lo;
+    split8(v, h, lo);
+    *reinterpret_cast<f16x8*>(d + at) = h;
+    *reinterpret_cast<f16x8*>(d + (int64_t)rows * ldk + at) = lo;
+  };
+  [[maybe_unused]] auto result_out = [&](int64_t at, int m, const float (&v)[8]) {  // m of the 8 values exist
     if constexpr (PHASE == kLast) {
-      if (tall == (turned == 1)) continue;  // G's own orientation only
-    }
-    if (PHASE <= kPoly && turned == 1 && ti == tj) continue;  // a diagonal tile is its own mirror image
-    const int r0 = turned ? i0 : j0, c0 = turned ? j0 : i0;
-    const int nr = PHASE <= kPoly ? k : turned ? k : n, nc = PHASE <= kPoly ? k : turned ? n : k;
-    const int ld = PHASE <= kPoly || !turned ? (int)l.ldk : (int)l.ldn;
-    for (int q = threadIdx.x; q < TT * PIECES; q += 256) {
-      const int r = q / PIECES, c = (q % PIECES) * 8;
-      if (r0 + r >= nr || c0 + c >= ld) continue;
-      float v[8];
-      if (turned) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[(c + e) * LDT + r];
-      } else {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + r * LDT + c), hi = *reinterpret_cast<const f32x4*>(tile + r * LDT + c + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
-      }
-      const int64_t at = (int64_t)(r0 + r) * ld + c0 + c;
-      if constexpr (PHASE >= kApply) {  // + a X, from X or X^T in this orientation (X is overwritten below by the thread that reads it)
-        const _Float16* X = reinterpret_cast<const _Float16*>(base + (turned ? l.x : xt_in));
-        const f16x8 h = *reinterpret_cast<const f16x8*>(X + at), lo = *reinterpret_cast<const f16x8*>(X + (int64_t)nr * ld + at);
-        const float fa = ldexpf(ca, PHASE == kApply ? eY - eX : -eX);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(fa, (float)h[e] + (float)lo[e], v[e]);
-      }
-      if constexpr (PHASE == kPoly) {  // + b A, then to B's scale
-        const _Float16* A = reinterpret_cast<const _Float16*>(base + l.a);
-        const f16x8 h = *reinterpret_cast<const f16x8*>(A + at), lo = *reinterpret_cast<const f16x8*>(A + (int64_t)k * ld + at);
-        const float fa = ldexpf(cb, -eA), fs = ldexpf(1.f, eB);
+      TO* d = static_cast<TO*>(to.dst[j]) + at;
+      if (m >= 8) {
+        typename Out8<TO>::type o;
+        if constexpr (MUON) o = *reinterpret_cast<typename Out8<TO>::type*>(d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = fmaf(fa, (float)h[e] + (float)lo[e], v[e]);
-          v[e] *= fs;
+          if constexpr (MUON) o[e] = fmaf(-mu.rate[j], v[e], o[e] * mu.keep);
+          else o[e] = (TO)v[e];
         }
-      }
-      if constexpr (PHASE != kLast) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c0 + c + e < nc ? v[e] : 0.f;  // the padding that the next product contracts over
-        _Float16* d = reinterpret_cast<_Float16*>(base + (PHASE == kGram ? l.a : PHASE == kPoly ? l.b : turned ? l.x : xt_out));
-        f16x8 h, lo;
-        split8(v, h, lo);
-        *reinterpret_cast<f16x8*>(d + at) = h;
-        *reinterpret_cast<f16x8*>(d + (int64_t)nr * ld + at) = lo;
+        *reinterpret_cast<typename Out8<TO>::type*>(d) = o;
       } else {
-        TO* d = static_cast<TO*>(jobs.dst[j]) + (int64_t)(r0 + r) * cols + c0 + c;
-        const int m = min(8, nc - (c0 + c));
-        if (m == 8) {
-          typename Out8<TO>::type o;
-          if constexpr (MUON) o = *reinterpret_cast<typename Out8<TO>::type*>(d);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if constexpr (MUON) o[e] = fmaf(-mu.rate[j], v[e], o[e] * mu.keep);
-            else o[e] = (TO)v[e];
-          }
-          *reinterpret_cast<typename Out8<TO>::type*>(d) = o;
-        } else {
-          for (int e = 0; e < m; ++e) {
-            if constexpr (MUON) d[e] = fmaf(-mu.rate[j], v[e], d[e] * mu.keep);
-            else d[e] = (TO)v[e];
-          }
+        for (int e = 0; e < 8; ++e) {
+          if (e >= m) break;
+          if constexpr (MUON) d[e] = fmaf(-mu.rate[j], v[e], d[e] * mu.keep);
+          else d[e] = (TO)v[e];
         }
       }
+    }
+  };
+  const bool again = PHASE <= kPoly ? ti != tj : PHASE == kLast && !job.tall;
+  _Float16* D = reinterpret_cast<_Float16*>(base + (PHASE == kGram ? l.a : PHASE == kPoly ? l.b : xt_out));
+#pragma unroll
+  for (int q = 0; q < MINE; ++q) {
+    const int r = (q * 256 + threadIdx.x) / PIECES, c = (threadIdx.x % PIECES) * 8;
+    float* p = tile + r * LDT + c;
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
+    if constexpr (PHASE != kGram) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(fe, (float)eh[q][e] + (float)el[q][e], v[e]);
+      if (again) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      }
+    }
+    if constexpr (PHASE != kLast) {
+      if (j0 + r < out_rows && i0 + c < ldk) {  // zeros beyond the matrix: the next products contract over them
+        const bool row_in = j0 + r < (PHASE <= kPoly ? k : n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = row_in && i0 + c + e < k ? v[e] : 0.f;
+        planes_out(D, out_rows, (int64_t)(j0 + r) * ldk + i0 + c, v);
+      }
+    } else if (!again && j0 + r < n) {
+      result_out((int64_t)(j0 + r) * k + i0 + c, k - (i0 + c), v);
+    }
+  }
+  if (!again) return;
+  if constexpr (PHASE != kGram) __syncthreads();
+#pragma unroll
+  for (int q = 0; q < MINE; ++q) {
+    const int r = (q * 256 + threadIdx.x) / PIECES, c = (threadIdx.x % PIECES) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[(c + e) * LDT + r];
+    if constexpr (PHASE <= kPoly) {
+      if (i0 + r < k && j0 + c < ldk) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = j0 + c + e < k ? v[e] : 0.f;
+        planes_out(D, k, (int64_t)(i0 + r) * ldk + j0 + c, v);
+      }
+    } else {
+      if (i0 + r < k) result_out((int64_t)(i0 + r) * n + j0 + c, n - (j0 + c), v);
     }
   }
 }
@@ -443,51 +615,45 @@ int tiles_of(int k, int n, bool symmetric) {
   const int64_t a = ceil_div(k, TT), b = ceil_div(n, TT);
   return (int)(symmetric ? a * (a + 1) / 2 : a * b);
 }
+template <typename Count>
+void place(Jobs& jobs, Count blocks_of) {
+  jobs.blocks = 0;
+  for (int j = 0; j < jobs.count; ++j) {
+    jobs.job[j].first = jobs.blocks;
+    jobs.blocks += blocks_of(jobs.job[j]);
+  }
+}
 
 template <int TT, int STAGES, int PHASE, typename TO, bool MUON>
-void launch_product(Jobs& jobs, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
-  int blocks = 0;
-  for (int j = 0; j < jobs.count; ++j) {
-    jobs.first[j] = blocks;
-    blocks += tiles_of<TT>(std::min(jobs.rows[j], jobs.cols[j]), std::max(jobs.rows[j], jobs.cols[j]), PHASE <= kPoly);
-  }
-  jobs.first[jobs.count] = blocks;
+void launch_product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
+  place(jobs, [](const Job& q) { return tiles_of<TT>(q.k, q.n, PHASE <= kPoly); });
   constexpr size_t lds = std::max<size_t>((size_t)STAGES * 4 * TT * kBK * 2, (size_t)TT * (TT + 4) * 4);
   const void* fn = (const void*)k_ns_product<TT, STAGES, PHASE, TO, MUON>;
   allow_big_lds(fn, lds);
-  hipLaunchKernelGGL((k_ns_product<TT, STAGES, PHASE, TO, MUON>), dim3(blocks), dim3(256), lds, st, jobs, mu, step, c[0], c[1], c[2]);
+  hipLaunchKernelGGL((k_ns_product<TT, STAGES, PHASE, TO, MUON>), dim3(jobs.blocks), dim3(256), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
 }
 
 template <int TT, int STAGES, typename TO, bool MUON>
-void run_steps(Jobs& jobs, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
+void run_steps(Jobs& jobs, const Results& to, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
+  const Nothing no{0};
   for (int t = 0; t < bd.steps; ++t) {
-    launch_product<TT, STAGES, kGram, float, false>(jobs, NoMuon{0}, t, bd.coef[t], st);
-    launch_product<TT, STAGES, kPoly, float, false>(jobs, NoMuon{0}, t, bd.coef[t], st);
-    if (t + 1 < bd.steps) launch_product<TT, STAGES, kApply, float, false>(jobs, NoMuon{0}, t, bd.coef[t], st);
-    else launch_product<TT, STAGES, kLast, TO, MUON>(jobs, mu, t, bd.coef[t], st);
+    launch_product<TT, STAGES, kGram, float, false>(jobs, no, no, t, bd.coef[t], st);
+    launch_product<TT, STAGES, kPoly, float, false>(jobs, no, no, t, bd.coef[t], st);
+    if (t + 1 < bd.steps) launch_product<TT, STAGES, kApply, float, false>(jobs, no, no, t, bd.coef[t], st);
+    else launch_product<TT, STAGES, kLast, TO, MUON>(jobs, to, mu, t, bd.coef[t], st);
   }
 }
 
 template <typename T, bool MUON>
-void run_chunk(Jobs& jobs, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
-  int blocks = 0;
-  for (int j = 0; j < jobs.count; ++j) {
-    jobs.first[j] = blocks;
-    blocks += (int)std::min<int64_t>(kMaxParts, ceil_div((int64_t)jobs.rows[j] * jobs.cols[j], kNormPart));
-  }
-  jobs.first[jobs.count] = blocks;
-  hipLaunchKernelGGL((k_ns_norm<T, MUON>), dim3(blocks), dim3(256), 0, st, jobs, mu);
-  blocks = 0;
+void run_chunk(Jobs& jobs, const Sources& from, const Results& to, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
+  place(jobs, [](const Job& q) { return parts_of(q.k, q.n); });
+  hipLaunchKernelGGL((k_ns_norm<T, MUON>), dim3(jobs.blocks), dim3(256), 0, st, jobs, from, mu);
+  place(jobs, [](const Job& q) { return tiles_of<64>(q.k, q.n, false); });
+  hipLaunchKernelGGL((k_ns_split<T, MUON>), dim3(jobs.blocks), dim3(256), 0, st, jobs, from, mu, bd);
   int64_t big = 0;
-  for (int j = 0; j < jobs.count; ++j) {
-    jobs.first[j] = blocks;
-    blocks += (int)(ceil_div(jobs.rows[j], 64) * ceil_div(jobs.cols[j], 64));
-    big += tiles_of<128>(std::min(jobs.rows[j], jobs.cols[j]), std::max(jobs.rows[j], jobs.cols[j]), true);
-  }
-  jobs.first[jobs.count] = blocks;
-  hipLaunchKernelGGL((k_ns_split<T, MUON>), dim3(blocks), dim3(256), 0, st, jobs, mu, bd);
-  if (big >= num_cu()) run_steps<128, 2, T, MUON>(jobs, mu, bd, st);
-  else run_steps<64, 4, T, MUON>(jobs, mu, bd, st);
+  for (int j = 0; j < jobs.count; ++j) big += tiles_of<128>(jobs.job[j].k, jobs.job[j].n, true);
+  if (big >= num_cu()) run_steps<128, 2, T, MUON>(jobs, to, mu, bd, st);
+  else run_steps<64, 4, T, MUON>(jobs, to, mu, bd, st);
 }
 
 // the matrices [from, to) of a chunk: at most kMaxJobs, and kChunkBytes unless one alone takes more
@@ -535,19 +701,20 @@ int run_all(const char* what, const int64_t* rows, const int64_t* cols, int64_t 
     size_t need;
     const int64_t to = chunk_end(rows, cols, from, count, need);
     Jobs jobs{};
+    Sources src{};
+    Results res{};
     MuonArgs mu{};
     jobs.ws = (char*)ws;
+    jobs.xcds = num_xcd();
     int64_t off = 0;
     for (int64_t j = from; j < to; ++j) {
       if (rows[j] == 0 || cols[j] == 0) continue;
       const int q = jobs.count++;
-      jobs.rows[q] = (int)rows[j];
-      jobs.cols[q] = (int)cols[j];
-      jobs.off[q] = off;
-      off += layout_of(std::min(rows[j], cols[j]), std::max(rows[j], cols[j])).bytes;
-      fill.set(jobs, mu, q, j);
+      jobs.job[q] = Job{0, (int)std::min(rows[j], cols[j]), (int)std::max(rows[j], cols[j]), rows[j] > cols[j], off};
+      off += layout_of(jobs.job[q].k, jobs.job[q].n).bytes;
+      fill.set(src, res, mu, q, j);
     }
-    if (jobs.count) fill.run(jobs, mu, bd);
+    if (jobs.count) fill.run(jobs, src, res, mu, bd);
     launched |= jobs.count > 0;
     from = to;
   }
@@ -555,35 +722,36 @@ int run_all(const char* what, const int64_t* rows, const int64_t* cols, int64_t 
 }
 
 struct FillPlain {
-  const void* const* src; const int64_t* ld; void* const* dst; const int64_t* cols; int type; hipStream_t st;
+  const void* const* src; const int64_t* ld; void* const* dst; int type; hipStream_t st;
   bool valid(int64_t j) const { return src[j] && dst[j] && ld[j] >= 0; }
-  void set(Jobs& jobs, MuonArgs&, int q, int64_t j) const {
-    jobs.src[q] = src[j];
-    jobs.dst[q] = dst[j];
-    jobs.ld[q] = ld[j];
+  void set(Sources& s, Results& r, MuonArgs&, int q, int64_t j) const {
+    s.src[q] = src[j];
+    s.ld[q] = ld[j];
+    r.dst[q] = dst[j];
   }
-  void run(Jobs& jobs, const MuonArgs&, const Bounds& bd) const {
-    if (type == PGNN_F32) run_chunk<float, false>(jobs, NoMuon{0}, bd, st);
-    else if (type == PGNN_BF16) run_chunk<__bf16, false>(jobs, NoMuon{0}, bd, st);
-    else run_chunk<_Float16, false>(jobs, NoMuon{0}, bd, st);
+  void run(Jobs& jobs, const Sources& s, const Results& r, const MuonArgs&, const Bounds& bd) const {
+    const Nothing no{0};
+    if (type == PGNN_F32) run_chunk<float, false>(jobs, s, r, no, bd, st);
+    else if (type == PGNN_BF16) run_chunk<__bf16, false>(jobs, s, r, no, bd, st);
+    else run_chunk<_Float16, false>(jobs, s, r, no, bd, st);
   }
 };
 struct FillMuon {
   float* const* params; const float* const* grads; float* const* momentum; const float* rates; const int64_t* cols; float mu, keep; int nesterov;
   hipStream_t st;
   bool valid(int64_t j) const { return params[j] && grads[j] && momentum[j]; }
-  void set(Jobs& jobs, MuonArgs& m, int q, int64_t j) const {
-    jobs.src[q] = grads[j];
-    jobs.dst[q] = params[j];
-    jobs.ld[q] = cols[j];
+  void set(Sources& s, Results& r, MuonArgs& m, int q, int64_t j) const {
+    s.src[q] = grads[j];
+    s.ld[q] = cols[j];
+    r.dst[q] = params[j];
     m.momentum[q] = momentum[j];
     m.rate[q] = rates[j];
   }
-  void run(Jobs& jobs, MuonArgs& m, const Bounds& bd) const {
+  void run(Jobs& jobs, const Sources& s, const Results& r, MuonArgs& m, const Bounds& bd) const {
     m.mu = mu;
     m.keep = keep;
     m.nesterov = nesterov;
-    run_chunk<float, true>(jobs, m, bd, st);
+    run_chunk<float, true>(jobs, s, r, m, bd, st);
   }
 };
 
@@ -607,7 +775,7 @@ int pgnn_newton_schulz(const void* const* src, const int64_t* ld_src, void* cons
   PGNN_REQUIRE(type == PGNN_F32 || type == PGNN_BF16 || type == PGNN_F16, "newton_schulz: type %d", type);
   PGNN_REQUIRE(count <= 0 || (src && ld_src && dst), "newton_schulz: bad list of matrices");
   return run_all("newton_schulz", rows, cols, count, coefficients, steps, eps, ws, ws_bytes,
-                 FillPlain{src, ld_src, dst, cols, type, (hipStream_t)stream});
+                 FillPlain{src, ld_src, dst, type, (hipStream_t)stream});
 }
 
 int pgnn_muon_step(float* const* params, const float* const* grads, float* const* momentum, const float* rates, const int64_t* rows,
