@@ -42,21 +42,41 @@ __host__ __device__ inline int parts_of(int64_t k, int64_t n) {
 
 // where a matrix's planes are in its part of the workspace (bytes): the exponents and the partial sums in front, at fixed places; planes
 // of 64 k columns are multiples of 256 bytes by themselves
-constexpr int64_t kExps = 0, kParts = 512, kPlanes = kParts + kMaxParts * 8;
-static_assert(3 * (kMaxSteps + 1) * 4 <= kParts && kPlanes % 256 == 0, "");
+constexpr int kExpRow = kMaxSteps + 1;  // exponents of X_t, A_t, B_t, Z_t: four rows
+constexpr int64_t kExps = 0, kParts = 768, kPlanes = kParts + kMaxParts * 8;
+static_assert(4 * kExpRow * 4 <= kParts && kPlanes % 256 == 0, "");
+// A matrix on planes lies in blocks of 16 rows x 32 columns, the high plane's 1 KB and then the low one's, down a column of blocks and then
+// the next (what a stage of a product takes of an operand is one piece).  Inside a block the lane (fr, fc) of a wave that takes it as an operand -- row fr, columns 8 fc .. 8 fc + 7 -- has the 16
+// bytes at unit_of(fr, fc): every fragment and every DMA is 1 KB in one piece (as 64- or 128-byte pieces of 16 rows of a row-major matrix
+// a CU took 18 to 27 bytes per clock of them), and LDS holds blocks as memory does.  The xor keeps both ways
+// of reading free of bank conflicts: ds_read_b128 takes rows 0-3 and 12-15 of one fc together with rows 4-11 of the next, and
+// ds_read_b64_tr_b16 takes rows 0-3 and 8-11 of two neighbours (an xor by 4 does for the second only: A A of 4096 x 4096 268 instead of 264 us).
+constexpr int kBlockHalfs = 1024;  // both planes
+__host__ __device__ inline int unit_of(int fr, int fc) { return fc * 16 + (fr ^ ((fc & 1) * 12)); }
 struct Layout {
-  int64_t ldk, rows, xt0, xt1, a, b, bytes;  // X^T: `rows` rows, n of them and zeros up to whole stages
+  int64_t ldk, rows, xt0, xt1, a, b, bytes;  // ldk: columns, and rows of A and B; rows: of X^T, n of them, then zeros
 };
 __host__ __device__ inline Layout layout_of(int64_t k, int64_t n) {
   Layout l;
   l.ldk = (k + kPad - 1) & ~(int64_t)(kPad - 1);
-  l.rows = (n + kBK - 1) & ~(int64_t)(kBK - 1);
+  l.rows = (n + kPad - 1) & ~(int64_t)(kPad - 1);
   l.xt0 = kPlanes;
   l.xt1 = l.xt0 + 4 * l.rows * l.ldk;
   l.a = l.xt1 + 4 * l.rows * l.ldk;
-  l.b = l.a + 4 * k * l.ldk;
-  l.bytes = l.b + 4 * k * l.ldk;
+  l.b = l.a + 4 * l.ldk * l.ldk;
+  l.bytes = l.b + 4 * l.ldk * l.ldk;
   return l;
+}
+// where the eight columns c .. c + 7 of row r begin (halfs, high plane)
+__device__ __forceinline__ int64_t piece_at(int rows, int r, int c) {
+  return ((int64_t)(c >> 5) * (rows >> 4) + (r >> 4)) * kBlockHalfs + unit_of(r & 15, (c >> 3) & 3) * 8;
+}
+// row and first column of piece p of a tile WIDE columns wide, in the order in which the pieces lie in memory
+template <int WIDE>
+__device__ __forceinline__ void piece_of(int p, int& r, int& c) {
+  const int block = p >> 6, fc = (p >> 4) & 3;
+  r = block / (WIDE / 32) * 16 + ((p & 15) ^ ((fc & 1) * 12));
+  c = block % (WIDE / 32) * 32 + fc * 8;
 }
 
 // a matrix of the call: its first workgroup in this launch, its sizes (k <= n), whether G has more rows than columns, its workspace
@@ -92,12 +112,22 @@ struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps
   float eps;
 };
 
-// the job of a workgroup, found by one vector load and a ballot: a bisection is a chain of scalar loads, each of which waits for the
-// kernel arguments anew
-__device__ __forceinline__ int find_job(const Jobs& jobs, int b) {
+// the job of a workgroup: every lane loads one, a ballot finds the last that begins at or before this workgroup, its fields are read from
+// that lane.  One round trip to the kernel arguments; a bisection and a load of what it found are five
+struct Found : Job { int index; };
+__device__ __forceinline__ Found find_job(const Jobs& jobs, int b) {
   const int lane = threadIdx.x & 63;
-  const int first = lane < jobs.count ? jobs.job[lane].first : 0x7fffffff;
-  return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(first <= b)) - 1);
+  const Job mine = jobs.job[min(lane, kMaxJobs - 1)];
+  const int at = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(lane < jobs.count && mine.first <= b)) - 1);
+  Found f;
+  f.index = at;
+  f.first = __builtin_amdgcn_readlane(mine.first, at);
+  f.k = __builtin_amdgcn_readlane(mine.k, at);
+  f.n = __builtin_amdgcn_readlane(mine.n, at);
+  f.tall = __builtin_amdgcn_readlane(mine.tall, at);
+  f.off = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine.off, at) |
+          (int64_t)__builtin_amdgcn_readlane((int)(mine.off >> 32), at) << 32;
+  return f;
 }
 // 16 bytes of G at the element's own alignment
 template <typename T> struct Piece { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); static constexpr int n = 16 / sizeof(T); };
@@ -105,8 +135,8 @@ template <typename T> struct Piece { typedef T type __attribute__((ext_vector_ty
 // partial sums of squares in float64 (millions of terms, squares of gradients far below 1); Muon: the momentum is advanced here
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) k_ns_norm(Jobs jobs, Sources from, Muon<MUON> mu) {
-  const int j = find_job(jobs, blockIdx.x);
-  const Job job = jobs.job[j];
+  const Found job = find_job(jobs, blockIdx.x);
+  const int j = job.index;
   const int rows = job.tall ? job.n : job.k, cols = job.tall ? job.k : job.n;
   const int nparts = parts_of(job.k, job.n), part = blockIdx.x - job.first;
   const T* g = static_cast<const T*>(from.src[j]);
@@ -178,8 +208,8 @@ __device__ __forceinline__ void split8(const float (&v)[8], f16x8& h, f16x8& l) 
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<MUON> mu, Bounds bd) {
   const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
-  const int j = find_job(jobs, b);
-  const Job job = jobs.job[j];
+  const Found job = find_job(jobs, b);
+  const int j = job.index;
   const bool tall = job.tall;
   const int rows = tall ? job.n : job.k, cols = tall ? job.k : job.n;
   const Layout l = layout_of(job.k, job.n);
@@ -205,9 +235,10 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
     for (int t = 0; t < bd.steps; ++t) {
       const float a = fabsf(bd.coef[t][0]), b = fabsf(bd.coef[t][1]), c = fabsf(bd.coef[t][2]);
       const float al = fmaxf(1.001f * u * u, 0x1p-60f);
-      e[kMaxSteps + 1 + t] = plane_exponent(al);                                                       // A
+      e[kExpRow + t] = plane_exponent(al);                                                       // A
       const float be = fmaxf(fminf(1.001f * al * (b + al * c), bd.cap_b[t]), 0x1p-60f);
-      e[2 * (kMaxSteps + 1) + t] = plane_exponent(be);                                                 // B
+      e[2 * kExpRow + t] = plane_exponent(be);                                                 // B
+      e[3 * kExpRow + t] = plane_exponent(fmaxf(1.001f * u * (b + al * c), 0x1p-60f));          // Z = b X + c A X
       u = fmaxf(fminf((a + be) * u, bd.cap_x[t + 1]), 0x1p-60f);
       e[t + 1] = plane_exponent(u);                                                                    // X
     }
@@ -252,8 +283,8 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
   const int dr0 = tall ? r0 : c0, dc0 = tall ? c0 : r0;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const int i = q * 256 + threadIdx.x, r = i >> 3, c = (i & 7) * 8;
-    if (dr0 + r >= (int)l.rows) continue;  // (rows n .. l.rows: zeros)
+    int r, c;
+    piece_of<64>(q * 256 + threadIdx.x, r, c);  // (rows n .. l.rows: zeros)
     float v[8];
     if (tall) {
 #pragma unroll
@@ -264,9 +295,9 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
     }
     f16x8 h, lo;
     split8(v, h, lo);
-    const int64_t at = (int64_t)(dr0 + r) * l.ldk + dc0 + c;
+    const int64_t at = piece_at((int)l.rows, dr0 + r, dc0 + c);
     *reinterpret_cast<f16x8*>(d + at) = h;
-    *reinterpret_cast<f16x8*>(d + l.rows * l.ldk + at) = lo;
+    *reinterpret_cast<f16x8*>(d + at + kBlockHalfs / 2) = lo;
   }
 }
 
@@ -300,21 +331,20 @@ __device__ __forceinline__ void tile_at(int local, int down, int across, bool sy
   }
 }
 
-// four blocks of 16 columns x 32 l, both planes, turned on their way out of LDS: at[b] the lane's address of block b, H the distance of
-// l + 4, ARR that of the low plane.  One asm block with its own wait: with the builtin hipcc waits for every DMA in flight in front of the
-// reads (ten 300 x 600: X X^T 15.7 us instead of 11.0), and a load of inline asm must not leave its block unfinished.
-template <int H, int ARR>
+// four blocks of 16 columns x 32 l, both planes, turned on their way out of LDS: at[b] the lane's address in block b's high plane, l + 4
+// is that xor 64, the low plane 1 KB further.  One asm block with its own wait: with the builtin hipcc waits for every DMA in flight in
+// front of the reads (ten 300 x 600: X X^T 15.7 us instead of 11.0), and a load of inline asm must not leave its block unfinished.
 __device__ __forceinline__ void read_turned(const uint32_t (&at)[4], f16x8 (&hi)[4], f16x8 (&lo)[4]) {
   uint2 r[4][4];
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%20\n\tds_read_b64_tr_b16 %2, %16 offset:%21\n\tds_read_b64_tr_b16 %3, %16 offset:%22\n\t"
-      "ds_read_b64_tr_b16 %4, %17\n\tds_read_b64_tr_b16 %5, %17 offset:%20\n\tds_read_b64_tr_b16 %6, %17 offset:%21\n\tds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
-      "ds_read_b64_tr_b16 %8, %18\n\tds_read_b64_tr_b16 %9, %18 offset:%20\n\tds_read_b64_tr_b16 %10, %18 offset:%21\n\tds_read_b64_tr_b16 %11, %18 offset:%22\n\t"
-      "ds_read_b64_tr_b16 %12, %19\n\tds_read_b64_tr_b16 %13, %19 offset:%20\n\tds_read_b64_tr_b16 %14, %19 offset:%21\n\tds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
+      "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %20\n\tds_read_b64_tr_b16 %2, %16 offset:1024\n\tds_read_b64_tr_b16 %3, %20 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %4, %17\n\tds_read_b64_tr_b16 %5, %21\n\tds_read_b64_tr_b16 %6, %17 offset:1024\n\tds_read_b64_tr_b16 %7, %21 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %8, %18\n\tds_read_b64_tr_b16 %9, %22\n\tds_read_b64_tr_b16 %10, %18 offset:1024\n\tds_read_b64_tr_b16 %11, %22 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %12, %19\n\tds_read_b64_tr_b16 %13, %23\n\tds_read_b64_tr_b16 %14, %19 offset:1024\n\tds_read_b64_tr_b16 %15, %23 offset:1024\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[0][2]), "=&v"(r[0][3]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[1][2]), "=&v"(r[1][3]),
         "=&v"(r[2][0]), "=&v"(r[2][1]), "=&v"(r[2][2]), "=&v"(r[2][3]), "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[3][2]), "=&v"(r[3][3])
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(H), "n"(ARR), "n"(ARR + H)
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[0] ^ 64u), "v"(at[1] ^ 64u), "v"(at[2] ^ 64u), "v"(at[3] ^ 64u)
       : "memory");
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
@@ -323,66 +353,57 @@ __device__ __forceinline__ void read_turned(const uint32_t (&at)[4], f16x8 (&hi)
   }
 }
 
-// One TT x TT tile of a product on planes, C[i][j] = sum_l P(i, l) Q(j, l).  Four waves of TT/2 x TT/2; wave w fetches operand array w
-// (P high, P low, Q high, Q low) by LDS DMA, STAGES - 1 stages ahead.  A stage is 32 deep.
-//   A A and B X: l runs along the operands' rows.  A stage holds 64 bytes of TT rows, whose four 16-byte pieces are permuted by
-//   (row >> 1) & 3, so that the eight rows of a piece that one LDS cycle reads lie in eight different bank groups.
-//   X X^T: l runs down the rows of X^T.  A stage holds 32 rows of 2 TT bytes; a fragment (8 l of one column per lane) is two
-//   ds_read_b64_tr_b16, each of which hands a 16-lane group a 4 x 16 block turned.  The 32-byte blocks of a row are permuted by bits of
-//   the row, so that the 16 rows that one instruction reads lie evenly over the banks.
+// One TT x TT tile of a product on planes, C[i][j] = sum_l P(i, l) Q(j, l).  Four waves of TT/2 x TT/2; two fetch P and two fetch Q by LDS
+// DMA, STAGES - 1 stages ahead.  A stage is 32 deep: of A A and B X, where l runs along the operands' rows, a column of TT/16 blocks of
+// each; of X X^T, where l runs down the rows of X^T, two rows of TT/32 blocks, whose fragments (8 l of one column per lane) are two
+// ds_read_b64_tr_b16 each: a 16-lane group hands over 4 rows x 16 columns turned.
 template <int TT, int STAGES, int PHASE, typename TO, bool MUON>
 __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
-  constexpr int MI = TT / 32, ARR = TT * kBK * 2, STAGE = 4 * ARR, NJ = TT / 16;
+  constexpr int MI = TT / 32, OPER = TT * kBK * 4, STAGE = 2 * OPER, NJ = TT / 16;
   constexpr int LDT = TT + 4;  // floats per row of the epilogue's tile: 16-byte rows, neighbours four banks apart
   extern __shared__ __align__(16) char smem[];
   const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
-  const int j = find_job(jobs, b);
-  const Job job = jobs.job[j];
+  const Found job = find_job(jobs, b);
+  const int j = job.index;
   const int k = job.k, n = job.n;
   const Layout l = layout_of(k, n);
   char* base = jobs.ws + job.off;
   int ti, tj;
   tile_at(b - job.first, (k + TT - 1) / TT, ((PHASE <= kPoly ? k : n) + TT - 1) / TT, PHASE <= kPoly, ti, tj);
   const int* exps = reinterpret_cast<const int*>(base + kExps);
-  const int eX = exps[step], eA = exps[kMaxSteps + 1 + step], eB = exps[2 * (kMaxSteps + 1) + step], eY = exps[step + 1];
+  const int eX = exps[step], eA = exps[kExpRow + step], eB = exps[2 * kExpRow + step], eY = exps[step + 1];
   const int64_t xt_in = step & 1 ? l.xt1 : l.xt0, xt_out = step & 1 ? l.xt0 : l.xt1;
   const _Float16* XT = reinterpret_cast<const _Float16*>(base + xt_in);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int i0 = ti * TT, j0 = tj * TT, ldk = (int)l.ldk;
 
-  // the wave's DMA pieces: 1 KB each
+  // the wave's DMA pieces: 1 KB each, NJ of its half of P (waves 0, 1) or Q (waves 2, 3)
   const _Float16* src;
-  uint32_t offs[NJ];  // in halfs; what lies beyond the matrix re-reads its last row or column (the results are not stored)
+  uint32_t offs[NJ];  // in halfs; blocks beyond the matrix's last are that one again (the results are not stored)
   int64_t advance;    // per stage
   int nk;
+  const int from = wave < 2 ? i0 : j0;
   if constexpr (PHASE == kGram) {
-    constexpr int UNITS = TT / 8, ROWS = 64 / UNITS;  // 16-byte units per row, rows per piece
-    src = XT + (wave & 1) * l.rows * ldk;
-    nk = (int)l.rows / kBK;
-    advance = (int64_t)kBK * ldk;
+    src = XT;
+    nk = (n + kBK - 1) / kBK;  // (k_ns_apply leaves rows behind the last strip as they are)
+    advance = 2 * kBlockHalfs;
 #pragma unroll
-    for (int q = 0; q < NJ; ++q) {
-      const int r = q * ROWS + lane / UNITS, u = lane % UNITS;
-      const int turn = TT == 64 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r & 3) | ((r >> 1) & 4);
-      const int col = (wave < 2 ? i0 : j0) + (((u >> 1) ^ turn) * 2 + (u & 1)) * 8;
-      offs[q] = (uint32_t)r * (uint32_t)ldk + (uint32_t)min(col, ldk - 8);
-    }
+    for (int q = 0; q < NJ; ++q)  // wave 0 / 2: the first row of blocks, 1 / 3: the second
+      offs[q] = (uint32_t)(min(from / 32 + (q >> 1), ldk / 32 - 1) * ((int)l.rows / 16) + (wave & 1)) * kBlockHalfs + (q & 1) * (kBlockHalfs / 2) + lane * 8;
   } else {
     const _Float16* P = reinterpret_cast<const _Float16*>(base + (PHASE == kPoly ? l.a : l.b));
-    const _Float16* Q = PHASE == kPoly ? P : XT;
-    const int qrows = PHASE == kPoly ? k : (int)l.rows;
-    src = wave < 2 ? P + (int64_t)(wave & 1) * k * ldk : Q + (int64_t)(wave & 1) * qrows * ldk;
+    src = wave < 2 || PHASE == kPoly ? P : XT;
+    const int down = (wave < 2 || PHASE == kPoly ? ldk : (int)l.rows) / 16;
     nk = ldk / kBK;
-    advance = kBK;
+    advance = (int64_t)down * kBlockHalfs;
 #pragma unroll
     for (int q = 0; q < NJ; ++q) {
-      const int r = q * 16 + (lane >> 2);
-      const int row = min((wave < 2 ? i0 : j0) + r, (wave < 2 ? k : qrows) - 1);
-      offs[q] = (uint32_t)row * (uint32_t)ldk + (uint32_t)(((lane & 3) ^ ((r >> 1) & 3)) * 8);
+      const int x = (wave & 1) * NJ + q;
+      offs[q] = (uint32_t)(min(from / 16 + (x >> 1), down - 1) * kBlockHalfs + (x & 1) * (kBlockHalfs / 2) + lane * 8);
     }
   }
   auto issue = [&](int t) {
-    char* dst = smem + (t % STAGES) * STAGE + wave * ARR;
+    char* dst = smem + (t % STAGES) * STAGE + wave * (OPER / 2);
 #pragma unroll
     for (int q = 0; q < NJ; ++q)
       __builtin_amdgcn_global_load_lds(PGNN_GPTR(src + (size_t)offs[q] + (size_t)t * advance), PGNN_LPTR(dst + q * 1024), 16, 0, 0);
@@ -390,17 +411,18 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
 
   // the epilogue's operand (A behind A A, X^T behind B X) at this thread's pieces of the tile, fetched in front of everything else: its
   // round trip to memory hides behind the product
-  constexpr int PIECES = TT / 8, MINE = TT * PIECES / 256;  // 16-byte pieces per row, pieces per thread
-  const int out_rows = PHASE <= kPoly ? k : (int)l.rows;
+  constexpr int MINE = TT * TT / 8 / 256;  // pieces of eight columns per thread
+  const int out_rows = PHASE <= kPoly ? ldk : (int)l.rows;
   [[maybe_unused]] f16x8 eh[MINE], el[MINE];
   if constexpr (PHASE != kGram) {
     const _Float16* E = PHASE == kPoly ? reinterpret_cast<const _Float16*>(base + l.a) : XT;
 #pragma unroll
     for (int q = 0; q < MINE; ++q) {
-      const int r = (q * 256 + threadIdx.x) / PIECES, c = (threadIdx.x % PIECES) * 8;
-      const int64_t at = (int64_t)min(j0 + r, out_rows - 1) * ldk + min(i0 + c, ldk - 8);
+      int r, c;
+      piece_of<TT>(q * 256 + threadIdx.x, r, c);
+      const int64_t at = piece_at(out_rows, min(j0 + r, out_rows - 1), min(i0 + c, ldk - 8));
       eh[q] = *reinterpret_cast<const f16x8*>(E + at);
-      el[q] = *reinterpret_cast<const f16x8*>(E + (int64_t)out_rows * ldk + at);
+      el[q] = *reinterpret_cast<const f16x8*>(E + at + kBlockHalfs / 2);
     }
   }
 
@@ -411,14 +433,16 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
 #pragma unroll
   for (int a = 0; a < MI; ++a) {
     const int pb = wi / 16 + a, qb = wj / 16 + a;
-    if constexpr (PHASE == kGram) {  // rows l = 8 fc + fr / 4; the rows l + 4 have the same permutation
-      const int r = 8 * fc + (fr >> 2);
-      const int turn = TT == 64 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r & 3) | ((r >> 1) & 4);
-      pat[a] = (uint32_t)(r * TT * 2 + (pb ^ turn) * 32 + (fr & 3) * 8);
-      qat[a] = (uint32_t)(r * TT * 2 + (qb ^ turn) * 32 + (fr & 3) * 8 + 2 * ARR);
+    if constexpr (PHASE == kGram) {  // row l = 8 fc + fr / 4, columns 4 (fr & 3) .. of the 16: unit 2 (block & 1) + (fr & 3) / 2 of that row
+      auto at = [&](int block) {
+        const int u = 2 * (block & 1) + ((fr & 3) >> 1);
+        return (uint32_t)(((fc >> 1) * (TT / 16) + (block >> 1) * 2) * 1024 + unit_of(8 * (fc & 1) + (fr >> 2), u) * 16 + (fr & 1) * 8);
+      };
+      pat[a] = at(pb);
+      qat[a] = at(qb) + OPER;
     } else {
-      pat[a] = (uint32_t)((pb * 16 + fr) * 64 + ((fc ^ ((fr >> 1) & 3)) * 16));
-      qat[a] = (uint32_t)((qb * 16 + fr) * 64 + ((fc ^ ((fr >> 1) & 3)) * 16) + 2 * ARR);
+      pat[a] = (uint32_t)(pb * 2048 + unit_of(fr, fc) * 16);
+      qat[a] = (uint32_t)(qb * 2048 + unit_of(fr, fc) * 16 + OPER);
     }
   }
 
@@ -445,21 +469,21 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
       const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)st;
       if constexpr (MI == 2) {
         f16x8 h[4], lo[4];
-        read_turned<4 * TT * 2, ARR>({at + pat[0], at + pat[1], at + qat[0], at + qat[1]}, h, lo);
+        read_turned({at + pat[0], at + pat[1], at + qat[0], at + qat[1]}, h, lo);
 #pragma unroll
         for (int a = 0; a < 2; ++a) { ph[a] = h[a]; pl[a] = lo[a]; qh[a] = h[2 + a]; ql[a] = lo[2 + a]; }
       } else {
         static_assert(MI == 2 || MI == 4, "");
-        read_turned<4 * TT * 2, ARR>({at + pat[0], at + pat[1], at + pat[2], at + pat[3]}, ph, pl);
-        read_turned<4 * TT * 2, ARR>({at + qat[0], at + qat[1], at + qat[2], at + qat[3]}, qh, ql);
+        read_turned({at + pat[0], at + pat[1], at + pat[2], at + pat[3]}, ph, pl);
+        read_turned({at + qat[0], at + qat[1], at + qat[2], at + qat[3]}, qh, ql);
       }
     } else {
 #pragma unroll
       for (int a = 0; a < MI; ++a) {
         ph[a] = *reinterpret_cast<const f16x8*>(st + pat[a]);
-        pl[a] = *reinterpret_cast<const f16x8*>(st + pat[a] + ARR);
+        pl[a] = *reinterpret_cast<const f16x8*>(st + pat[a] + 1024);
         qh[a] = *reinterpret_cast<const f16x8*>(st + qat[a]);
-        ql[a] = *reinterpret_cast<const f16x8*>(st + qat[a] + ARR);
+        ql[a] = *reinterpret_cast<const f16x8*>(st + qat[a] + 1024);
       }
     }
 #pragma unroll
@@ -488,11 +512,12 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
       *reinterpret_cast<f32x4*>(tile + (wj + c * 16 + fr) * LDT + wi + a * 16 + fc * 4) = acc[a][c] * f;
   __syncthreads();
 
-  auto planes_out = [&](_Float16* d, int rows, int64_t at, const float (&v)[8]) {
+  auto planes_out = [&](_Float16* d, int r, int c, const float (&v)[8]) {
     f16x8 h, lo;
     split8(v, h, lo);
+    const int64_t at = piece_at(out_rows, r, c);
     *reinterpret_cast<f16x8*>(d + at) = h;
-    *reinterpret_cast<f16x8*>(d + (int64_t)rows * ldk + at) = lo;
+    *reinterpret_cast<f16x8*>(d + at + kBlockHalfs / 2) = lo;
   };
   [[maybe_unused]] auto result_out = [&](int64_t at, int m, const float (&v)[8]) {  // m of the 8 values exist
     if constexpr (PHASE == kLast) {
@@ -508,11 +533,11 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
         *reinterpret_cast<typename Out8<TO>::type*>(d) = o;
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e >= m) break;
-          if constexpr (MUON) d[e] = fmaf(-mu.rate[j], v[e], d[e] * mu.keep);
-          else d[e] = (TO)v[e];
-        }
+        for (int e = 0; e < 8; ++e)
+          if (e < m) {
+            if constexpr (MUON) d[e] = fmaf(-mu.rate[j], v[e], d[e] * mu.keep);
+            else d[e] = (TO)v[e];
+          }
       }
     }
   };
@@ -520,7 +545,8 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
   _Float16* D = reinterpret_cast<_Float16*>(base + (PHASE == kGram ? l.a : PHASE == kPoly ? l.b : xt_out));
 #pragma unroll
   for (int q = 0; q < MINE; ++q) {
-    const int r = (q * 256 + threadIdx.x) / PIECES, c = (threadIdx.x % PIECES) * 8;
+    int r, c;
+    piece_of<TT>(q * 256 + threadIdx.x, r, c);
     float* p = tile + r * LDT + c;
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
     float v[8];
@@ -539,7 +565,7 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
         const bool row_in = j0 + r < (PHASE <= kPoly ? k : n);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = row_in && i0 + c + e < k ? v[e] : 0.f;
-        planes_out(D, out_rows, (int64_t)(j0 + r) * ldk + i0 + c, v);
+        planes_out(D, j0 + r, i0 + c, v);
       }
     } else if (!again && j0 + r < n) {
       result_out((int64_t)(j0 + r) * k + i0 + c, k - (i0 + c), v);
@@ -549,7 +575,8 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
   if constexpr (PHASE != kGram) __syncthreads();
 #pragma unroll
   for (int q = 0; q < MINE; ++q) {
-    const int r = (q * 256 + threadIdx.x) / PIECES, c = (threadIdx.x % PIECES) * 8;
+    int r, c;
+    piece_of<TT>(q * 256 + threadIdx.x, r, c);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[(c + e) * LDT + r];
@@ -557,11 +584,165 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
       if (i0 + r < k && j0 + c < ldk) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = j0 + c + e < k ? v[e] : 0.f;
-        planes_out(D, k, (int64_t)(i0 + r) * ldk + j0 + c, v);
+        planes_out(D, i0 + r, j0 + c, v);
       }
     } else {
       if (i0 + r < k) result_out((int64_t)(i0 + r) * n + j0 + c, n - (j0 + c), v);
     }
+  }
+}
+
+// The second half of a step for small k in one launch: X <- a X + A Z, Z = b X + c A X, a strip of 32 rows of X^T per workgroup (one row of
+// X^T knows nothing of another, so the two products need no exchange between workgroups; B = b A + c A A would, and one more launch).  It
+// costs 4 k^2 n instead of 2 k^3 + 2 k^2 n operations, which a small matrix has to spare: its launches are bound by their latency.
+// The strip and Z lie in LDS, A streams from L2 straight into registers -- every wave
+// takes whole 16-row blocks of A, so nothing of A is read twice by a workgroup -- kRing pairs of 32-deep steps ahead.  A lane's four results
+// are four consecutive columns of one row of X^T: they go to LDS as they are, and the strip leaves in whole rows.
+constexpr int kStrip = 32, kRing = 4, kSmall = 512;  // kSmall: two strips in 128 KB of LDS
+
+template <bool LAST, typename TO, bool MUON>
+__global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast : kApply> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
+  extern __shared__ __align__(16) char smem[];
+  const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
+  const Found job = find_job(jobs, b);
+  const int k = job.k, n = job.n;
+  const Layout l = layout_of(k, n);
+  char* base = jobs.ws + job.off;
+  const int j0 = (b - job.first) * kStrip, ldk = (int)l.ldk, down = (int)l.rows / 16;
+  const int* exps = reinterpret_cast<const int*>(base + kExps);
+  const int eX = exps[step], eA = exps[kExpRow + step], eZ = exps[3 * kExpRow + step], eY = exps[step + 1];
+  const _Float16* XT = reinterpret_cast<const _Float16*>(base + (step & 1 ? l.xt1 : l.xt0));
+  const _Float16* A = reinterpret_cast<const _Float16*>(base + l.a);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, nwaves = blockDim.x >> 6;
+  char* const strip = smem;
+  char* const zed = smem + kStrip * ldk * 4;
+
+  // the strip by DMA: 4 KB of each column of blocks
+  const _Float16* from = XT + (int64_t)(j0 / 16) * kBlockHalfs + lane * 8;
+  for (int q = wave; q < ldk / 8; q += nwaves)
+    __builtin_amdgcn_global_load_lds(PGNN_GPTR(from + (int64_t)(q >> 2) * down * kBlockHalfs + (q & 3) * 512), PGNN_LPTR(strip + q * 1024), 16, 0, 0);
+  const int fr = lane & 15, fc = lane >> 4;
+  const int pairs = ldk / 64;                                              // of 32-deep steps
+  const int blocks = wave < ldk / 16 ? (ldk / 16 - wave + nwaves - 1) / nwaves : 0;  // 16-row blocks of A for this wave
+  const int total = blocks * pairs;
+  f16x8 ring[kRing][4];  // high and low plane of two steps
+  int fblk = 0, fpr = 0;  // the next pair to fetch.  Past the end it stays on the last one: a load that is always issued leaves hipcc its count
+  auto fetch = [&](f16x8 (&d)[4]) {
+    const _Float16* s = A + ((int64_t)fpr * 2 * (ldk / 16) + min(wave + fblk * nwaves, ldk / 16 - 1)) * kBlockHalfs + unit_of(fr, fc) * 8;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = *reinterpret_cast<const f16x8*>(s + (int64_t)(e >> 1) * (ldk / 16) * kBlockHalfs + 512 * (e & 1));
+    if (fpr + 1 < pairs) {
+      ++fpr;
+    } else if (fblk + 1 < blocks) {
+      ++fblk;
+      fpr = 0;
+    }
+  };
+  auto prime = [&]() {
+    fblk = fpr = 0;
+#pragma unroll
+    for (int q = 0; q < kRing; ++q) fetch(ring[q]);
+  };
+  // C[i][j] = sum_l A[i][l] op[j][l] for the wave's blocks of rows i; done(i0, acc) per block
+  auto product = [&](const char* op, auto done) {
+    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    int blk = 0, pr = 0;
+    for (int at0 = 0; at0 < total; at0 += kRing) {
+#pragma unroll
+      for (int q = 0; q < kRing; ++q) {
+        if (at0 + q >= total) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f16x8 oh[2], ol[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const char* p = op + ((pr * 2 + h) * 2 + c) * 2048 + unit_of(fr, fc) * 16;
+            oh[c] = *reinterpret_cast<const f16x8*>(p);
+            ol[c] = *reinterpret_cast<const f16x8*>(p + 1024);
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h], ol[c], acc[c], 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h + 1], oh[c], acc[c], 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h], oh[c], acc[c], 0, 0, 0);
+        }
+        fetch(ring[q]);
+        if (++pr == pairs) {
+          done((wave + blk * nwaves) * 16, acc);
+          acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+          pr = 0;
+          ++blk;
+        }
+      }
+    }
+  };
+  // the lane's four columns i .. i + 3 of row r of an LDS operand
+  auto quad = [&](char* op, int r, int i, int low) {
+    return op + ((i >> 5) * 2 + (r >> 4)) * 2048 + low * 1024 + unit_of(r & 15, (i >> 3) & 3) * 16 + (i & 7) * 2;
+  };
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  auto x_at = [&](int r, int i, float (&x)[4]) {
+    const f16x4 h = *reinterpret_cast<const f16x4*>(quad(strip, r, i, 0)), lo = *reinterpret_cast<const f16x4*>(quad(strip, r, i, 1));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (float)h[e] + (float)lo[e];
+  };
+  auto put = [&](char* op, int r, int i, const float (&v)[4]) {
+    uint32_t h[2], lo[2];
+    split2(i < k ? v[0] : 0.f, i + 1 < k ? v[1] : 0.f, h[0], lo[0]);
+    split2(i + 2 < k ? v[2] : 0.f, i + 3 < k ? v[3] : 0.f, h[1], lo[1]);
+    *reinterpret_cast<uint2*>(quad(op, r, i, 0)) = make_uint2(h[0], h[1]);
+    *reinterpret_cast<uint2*>(quad(op, r, i, 1)) = make_uint2(lo[0], lo[1]);
+  };
+
+  prime();
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the strip (and the first of A); the builtin, which hipcc counts along with
+  __syncthreads();
+  {
+    const float fy = ldexpf(cc, eZ - eA - eX), fx = ldexpf(cb, eZ - eX);
+    product(strip, [&](int i0, const f32x4 (&acc)[2]) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = c * 16 + fr, i = i0 + 4 * fc;
+        float x[4], z[4];
+        x_at(r, i, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = fmaf(fx, x[e], acc[c][e] * fy);
+        put(zed, r, i, z);
+      }
+    });
+  }
+  prime();
+  __syncthreads();
+  const float fy = ldexpf(1.f, (LAST ? 0 : eY) - eA - eZ), fx = ldexpf(ca, (LAST ? 0 : eY) - eX);
+  product(zed, [&](int i0, const f32x4 (&acc)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = c * 16 + fr, i = i0 + 4 * fc;
+      float x[4], v[4];
+      x_at(r, i, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(fx, x[e], acc[c][e] * fy);
+      if constexpr (!LAST) {
+        put(strip, r, i, v);  // nobody else reads these four any more
+      } else if (j0 + r < n) {
+        const int64_t at = job.tall ? (int64_t)(j0 + r) * k + i : (int64_t)i * n + j0 + r, next = job.tall ? 1 : n;
+        TO* d = static_cast<TO*>(to.dst[job.index]) + at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (i + e >= k) break;
+          if constexpr (MUON) d[e * next] = fmaf(-mu.rate[job.index], v[e], d[e * next] * mu.keep);
+          else d[e * next] = (TO)v[e];
+        }
+      }
+    }
+  });
+  if constexpr (!LAST) {
+    __syncthreads();
+    _Float16* out = reinterpret_cast<_Float16*>(base + (step & 1 ? l.xt0 : l.xt1));
+    f16x8* d = reinterpret_cast<f16x8*>(out + (int64_t)(j0 / 16) * kBlockHalfs);
+    for (int q = threadIdx.x; q < kStrip * ldk / 4; q += blockDim.x)
+      d[(int64_t)(q >> 8) * down * (kBlockHalfs / 8) + (q & 255)] = reinterpret_cast<const f16x8*>(strip)[q];
   }
 }
 
@@ -633,11 +814,32 @@ void launch_product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int
   hipLaunchKernelGGL((k_ns_product<TT, STAGES, PHASE, TO, MUON>), dim3(jobs.blocks), dim3(256), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
 }
 
+template <bool LAST, typename TO, bool MUON>
+void launch_apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<MUON>& mu, int step, const float* c, int most, hipStream_t st) {
+  place(jobs, [](const Job& q) { return (int)ceil_div(q.n, kStrip); });
+  const int blocks = (int)layout_of(most, most).ldk / 16, each = (int)ceil_div(blocks, 8), waves = (int)ceil_div(blocks, each);
+  const size_t lds = (size_t)layout_of(most, most).ldk * kStrip * 8;
+  allow_big_lds((const void*)k_ns_apply<LAST, TO, MUON>, lds);
+  hipLaunchKernelGGL((k_ns_apply<LAST, TO, MUON>), dim3(jobs.blocks), dim3(64 * waves), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
+}
+
 template <int TT, int STAGES, typename TO, bool MUON>
 void run_steps(Jobs& jobs, const Results& to, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
   const Nothing no{0};
+  int most = 0;
+  int64_t strips = 0;
+  for (int j = 0; j < jobs.count; ++j) {
+    most = std::max(most, jobs.job[j].k);
+    strips += ceil_div(jobs.job[j].n, kStrip);
+  }
+  const bool small = most <= kSmall && strips <= num_cu();
   for (int t = 0; t < bd.steps; ++t) {
     launch_product<TT, STAGES, kGram, float, false>(jobs, no, no, t, bd.coef[t], st);
+    if (small) {
+      if (t + 1 < bd.steps) launch_apply<false, float, false>(jobs, no, no, t, bd.coef[t], most, st);
+      else launch_apply<true, TO, MUON>(jobs, to, mu, t, bd.coef[t], most, st);
+      continue;
+    }
     launch_product<TT, STAGES, kPoly, float, false>(jobs, no, no, t, bd.coef[t], st);
     if (t + 1 < bd.steps) launch_product<TT, STAGES, kApply, float, false>(jobs, no, no, t, bd.coef[t], st);
     else launch_product<TT, STAGES, kLast, TO, MUON>(jobs, to, mu, t, bd.coef[t], st);
