@@ -596,11 +596,12 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
 // X^T knows nothing of another, so the two products need no exchange between workgroups; B = b A + c A A would, and one more launch).  It
 // costs 4 k^2 n instead of 2 k^3 + 2 k^2 n operations, which a small matrix has to spare: its launches are bound by their latency.
 // The strip and Z lie in LDS, A streams from L2 straight into registers -- every wave
-// takes whole 16-row blocks of A, so nothing of A is read twice by a workgroup -- kRing pairs of 32-deep steps ahead.  A lane's four results
+// takes whole 16-row blocks of A, so nothing of A is read twice by a workgroup -- RING pairs of 32-deep steps ahead; the strip's
+// fragments of a pair are read from LDS while the pair before it multiplies.  A lane's four results
 // are four consecutive columns of one row of X^T: they go to LDS as they are, and the strip leaves in whole rows.
-constexpr int kStrip = 32, kRing = 4, kSmall = 512;  // kSmall: two strips in 128 KB of LDS
+constexpr int kStrip = 32, kSmall = 512;  // kSmall: two strips in 128 KB of LDS
 
-template <bool LAST, typename TO, bool MUON>
+template <int RING, bool LAST, typename TO, bool MUON>
 __global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast : kApply> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
   extern __shared__ __align__(16) char smem[];
   const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast :
   const int pairs = ldk / 64;                                              // of 32-deep steps
   const int blocks = wave < ldk / 16 ? (ldk / 16 - wave + nwaves - 1) / nwaves : 0;  // 16-row blocks of A for this wave
   const int total = blocks * pairs;
-  f16x8 ring[kRing][4];  // high and low plane of two steps
+  f16x8 ring[RING][4];  // high and low plane of two steps
   int fblk = 0, fpr = 0;  // the next pair to fetch.  Past the end it stays on the last one: a load that is always issued leaves hipcc its count
   auto fetch = [&](f16x8 (&d)[4]) {
     const _Float16* s = A + ((int64_t)fpr * 2 * (ldk / 16) + min(wave + fblk * nwaves, ldk / 16 - 1)) * kBlockHalfs + unit_of(fr, fc) * 8;
@@ -641,39 +642,47 @@ __global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast :
   auto prime = [&]() {
     fblk = fpr = 0;
 #pragma unroll
-    for (int q = 0; q < kRing; ++q) fetch(ring[q]);
+    for (int q = 0; q < RING; ++q) fetch(ring[q]);
   };
   // C[i][j] = sum_l A[i][l] op[j][l] for the wave's blocks of rows i; done(i0, acc) per block
   auto product = [&](const char* op, auto done) {
-    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-    int blk = 0, pr = 0;
-    for (int at0 = 0; at0 < total; at0 += kRing) {
+    f32x4 big[2], cross[2];  // high x high, and the two small terms: twice as many chains of dependent MFMAs
 #pragma unroll
-      for (int q = 0; q < kRing; ++q) {
-        if (at0 + q >= total) break;
+    for (int c = 0; c < 2; ++c) big[c] = cross[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f16x8 of[2][8];  // fragments of the strip for a pair: [step][block of 16][plane]
+    auto read = [&](int pr, f16x8 (&d)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = *reinterpret_cast<const f16x8*>(op + (pr * 4 + (e >> 1)) * 2048 + (e & 1) * 1024 + unit_of(fr, fc) * 16);
+    };
+    int blk = 0, pr = 0;
+    read(0, of[0]);
+    for (int at0 = 0; at0 < total; at0 += RING) {
+#pragma unroll
+      for (int q = 0; q < RING; ++q) {
+        const int next = pr + 1 == pairs ? 0 : pr + 1;
+        read(next, of[(q + 1) & 1]);
+        const f16x8 (&f)[8] = of[q & 1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          f16x8 oh[2], ol[2];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const char* p = op + ((pr * 2 + h) * 2 + c) * 2048 + unit_of(fr, fc) * 16;
-            oh[c] = *reinterpret_cast<const f16x8*>(p);
-            ol[c] = *reinterpret_cast<const f16x8*>(p + 1024);
-          }
+          for (int c = 0; c < 2; ++c) cross[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h], f[4 * h + 2 * c + 1], cross[c], 0, 0, 0);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h], ol[c], acc[c], 0, 0, 0);
+          for (int c = 0; c < 2; ++c) big[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h], f[4 * h + 2 * c], big[c], 0, 0, 0);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h + 1], oh[c], acc[c], 0, 0, 0);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h], oh[c], acc[c], 0, 0, 0);
+          for (int c = 0; c < 2; ++c) cross[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[q][2 * h + 1], f[4 * h + 2 * c], cross[c], 0, 0, 0);
         }
         fetch(ring[q]);
-        if (++pr == pairs) {
-          done((wave + blk * nwaves) * 16, acc);
-          acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-          pr = 0;
+        // (a whole ring is always run, the last one's surplus into nothing: with a way out between the slots hipcc waits for every load
+        // in flight at the head of the loop)
+        if (next == 0) {
+          big[0] += cross[0];
+          big[1] += cross[1];
+          if (blk < blocks) done((wave + blk * nwaves) * 16, big);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) big[c] = cross[c] = f32x4{0.f, 0.f, 0.f, 0.f};
           ++blk;
         }
+        pr = next;
       }
     }
   };
@@ -814,13 +823,13 @@ void launch_product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int
   hipLaunchKernelGGL((k_ns_product<TT, STAGES, PHASE, TO, MUON>), dim3(jobs.blocks), dim3(256), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
 }
 
-template <bool LAST, typename TO, bool MUON>
+template <int RING, bool LAST, typename TO, bool MUON>
 void launch_apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<MUON>& mu, int step, const float* c, int most, hipStream_t st) {
   place(jobs, [](const Job& q) { return (int)ceil_div(q.n, kStrip); });
   const int blocks = (int)layout_of(most, most).ldk / 16, each = (int)ceil_div(blocks, 8), waves = (int)ceil_div(blocks, each);
   const size_t lds = (size_t)layout_of(most, most).ldk * kStrip * 8;
-  allow_big_lds((const void*)k_ns_apply<LAST, TO, MUON>, lds);
-  hipLaunchKernelGGL((k_ns_apply<LAST, TO, MUON>), dim3(jobs.blocks), dim3(64 * waves), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
+  allow_big_lds((const void*)k_ns_apply<RING, LAST, TO, MUON>, lds);
+  hipLaunchKernelGGL((k_ns_apply<RING, LAST, TO, MUON>), dim3(jobs.blocks), dim3(64 * waves), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
 }
 
 template <int TT, int STAGES, typename TO, bool MUON>
@@ -836,8 +845,14 @@ void run_steps(Jobs& jobs, const Results& to, const Muon<MUON>& mu, const Bounds
   for (int t = 0; t < bd.steps; ++t) {
     launch_product<TT, STAGES, kGram, float, false>(jobs, no, no, t, bd.coef[t], st);
     if (small) {
-      if (t + 1 < bd.steps) launch_apply<false, float, false>(jobs, no, no, t, bd.coef[t], most, st);
-      else launch_apply<true, TO, MUON>(jobs, to, mu, t, bd.coef[t], most, st);
+      // (k <= 128: a wave has two pairs of steps in all)
+      if (t + 1 < bd.steps) {
+        if (most <= 128) launch_apply<2, false, float, false>(jobs, no, no, t, bd.coef[t], most, st);
+        else launch_apply<4, false, float, false>(jobs, no, no, t, bd.coef[t], most, st);
+      } else {
+        if (most <= 128) launch_apply<2, true, TO, MUON>(jobs, to, mu, t, bd.coef[t], most, st);
+        else launch_apply<4, true, TO, MUON>(jobs, to, mu, t, bd.coef[t], most, st);
+      }
       continue;
     }
     launch_product<TT, STAGES, kPoly, float, false>(jobs, no, no, t, bd.coef[t], st);
