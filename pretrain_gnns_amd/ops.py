@@ -800,7 +800,8 @@ def _call_workspace(nbytes, device):
 def _last_axis_rows(t, dim):
     """[rows, dim] view of a tensor whose trailing axes hold ``dim`` values, columns contiguous (any row stride); a copy where the
     strides allow no view"""
-    t = t.reshape(-1, dim) if t.numel() else t.new_empty(0, dim)
+    if t.dim() != 2 or t.size(1) != dim:
+        t = t.reshape(-1, dim) if t.numel() else t.new_empty(0, dim)
     return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
 
 
@@ -810,12 +811,41 @@ def _layer_norm_fwd(x, gamma, beta, dim, eps, relu, keep):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
     mean = stats.data_ptr() if keep and rows else None
-    wt = gamma if gamma is not None else beta
-    check(load().pgnn_layer_norm_fwd(rows2d.data_ptr(), rows2d.stride(0), gamma.data_ptr() if gamma is not None else None,
-                                     beta.data_ptr() if beta is not None else None, eps, relu, y.data_ptr(), dim, mean,
-                                     mean + 4 * rows if mean else None, rows, dim, _TYPE_CODES[x.dtype],
-                                     _TYPE_CODES[wt.dtype if wt is not None else x.dtype], stream_ptr()), "pgnn_layer_norm_fwd")
+    wt = gamma if gamma is not None else beta if beta is not None else x
+    rc = load().pgnn_layer_norm_fwd(rows2d.data_ptr(), rows2d.stride(0), gamma.data_ptr() if gamma is not None else None,
+                                    beta.data_ptr() if beta is not None else None, eps, relu, y.data_ptr(), dim, mean,
+                                    mean + 4 * rows if mean else None, rows, dim, _TYPE_CODES[x.dtype], _TYPE_CODES[wt.dtype],
+                                    stream_ptr(x.device.index))
+    if rc:
+        check(rc, "pgnn_layer_norm_fwd")
     return y, rows2d, stats
+
+
+def _layer_norm_bwd(ctx, dy):
+    x, gamma, beta, stats = ctx.saved_tensors
+    dim, rows, dev = ctx.dim, x.size(0), x.device
+    dy = _last_axis_rows(dy, dim)
+    need = ctx.needs_input_grad
+    dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if need[0] else None
+    dgamma = torch.empty(gamma.shape, dtype=gamma.dtype, device=dev) if need[1] and gamma is not None else None
+    dbeta = torch.empty(beta.shape, dtype=beta.dtype, device=dev) if need[2] and beta is not None else None
+    ws = ws_bytes = None
+    if dgamma is not None or dbeta is not None:
+        buf = _call_workspace(_ws_bytes("pgnn_layer_norm_bwd_workspace_bytes", rows, dim), dev)
+        ws, ws_bytes = buf.data_ptr(), buf.numel()
+    wt = gamma if gamma is not None else beta if beta is not None else x
+    mean = stats.data_ptr()
+    rc = load().pgnn_layer_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), gamma.data_ptr() if gamma is not None else None,
+                                    beta.data_ptr() if beta is not None else None, mean, mean + 4 * rows, ctx.relu,
+                                    dx.data_ptr() if dx is not None else None, dim, dgamma.data_ptr() if dgamma is not None else None,
+                                    dbeta.data_ptr() if dbeta is not None else None, rows, dim, _TYPE_CODES[x.dtype], _TYPE_CODES[wt.dtype],
+                                    ws, ws_bytes or 0, stream_ptr(dev.index))
+    if rc:
+        check(rc, "pgnn_layer_norm_bwd")
+    return dx, dgamma, dbeta, None, None, None
+
+
+_layer_norm_bwd_once = once_differentiable(_layer_norm_bwd)
 
 
 class LayerNormReLU(Function):
@@ -823,33 +853,15 @@ class LayerNormReLU(Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, dim, eps, relu):
-        with _on_device(x.device):
-            y, rows2d, stats = _layer_norm_fwd(x, gamma, beta, dim, eps, relu, True)
+        y, rows2d, stats = _layer_norm_fwd(x, gamma, beta, dim, eps, relu, True)
         ctx.save_for_backward(rows2d, gamma, beta, stats)
         ctx.dim, ctx.relu, ctx.shape = dim, relu, x.shape
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, gamma, beta, stats = ctx.saved_tensors
-        dim, rows = ctx.dim, x.size(0)
-        with _on_device(x.device):
-            dy = _last_axis_rows(dy, dim)
-            need_x, need_g, need_b = ctx.needs_input_grad[:3]
-            dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device) if need_x else None
-            dgamma = torch.empty(gamma.shape, dtype=gamma.dtype, device=x.device) if need_g and gamma is not None else None
-            dbeta = torch.empty(beta.shape, dtype=beta.dtype, device=x.device) if need_b and beta is not None else None
-            ws = None
-            if dgamma is not None or dbeta is not None:
-                ws = _call_workspace(_ws_bytes("pgnn_layer_norm_bwd_workspace_bytes", rows, dim), x.device)
-            wt = gamma if gamma is not None else beta
-            ptr = lambda t: t.data_ptr() if t is not None else None
-            check(load().pgnn_layer_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), ptr(gamma), ptr(beta), stats.data_ptr(),
-                                             stats.data_ptr() + 4 * rows, ctx.relu, ptr(dx), dim, ptr(dgamma), ptr(dbeta), rows, dim,
-                                             _TYPE_CODES[x.dtype], _TYPE_CODES[wt.dtype if wt is not None else x.dtype], ptr(ws),
-                                             ws.numel() if ws is not None else 0, stream_ptr()), "pgnn_layer_norm_bwd")
-        return dx, dgamma, dbeta, None, None, None
+        # (once_differentiable's wrapper costs as much as the call: it is needed where a graph of the backward is asked for)
+        return _layer_norm_bwd_once(ctx, dy) if torch.is_grad_enabled() else _layer_norm_bwd(ctx, dy)
 
 
 def layer_norm(x, ln, relu=False):
@@ -859,29 +871,39 @@ def layer_norm(x, ln, relu=False):
     up in a fixed order."""
     gamma, beta = ln.weight, ln.bias
     require_cuda(x, gamma, beta)
-    shape = tuple(ln.normalized_shape)
-    if x.dim() < len(shape) or tuple(x.shape[x.dim() - len(shape):]) != shape:
-        raise ValueError("layer_norm: expected trailing axes %s, got input size %s" % (shape, tuple(x.shape)))
-    if x.dtype not in _TYPE_CODES:
-        raise _lib.PgnnError("layer_norm: rows of fp32, bf16 or fp16, got %s" % x.dtype)
+    shape = ln.normalized_shape
+    if len(shape) == 1:
+        dim = shape[0]
+        fits = x.dim() >= 1 and x.size(-1) == dim
+    else:
+        dim = 1
+        for k in shape:
+            dim *= k
+        fits = x.dim() >= len(shape) and tuple(x.shape[x.dim() - len(shape):]) == tuple(shape)
+    if not fits:
+        raise ValueError("layer_norm: expected trailing axes %s, got input size %s" % (tuple(shape), tuple(x.shape)))
+    if dim == 0:
+        raise ValueError("layer_norm: nothing to normalise over in %s" % (tuple(shape),))
+    dtype = x.dtype
+    if dtype not in _TYPE_CODES:
+        raise _lib.PgnnError("layer_norm: rows of fp32, bf16 or fp16, got %s" % dtype)
     for t in (gamma, beta):
         if t is None:
             continue
-        if t.dtype not in (x.dtype, torch.float32) or t.dtype != (gamma if gamma is not None else beta).dtype:
-            raise _lib.PgnnError("layer_norm: gains of the rows' type (%s) or float32, both of one type, got %s" % (x.dtype, t.dtype))
+        if (t.dtype is not dtype and t.dtype is not torch.float32) or (gamma is not None and t.dtype is not gamma.dtype):
+            raise _lib.PgnnError("layer_norm: gains of the rows' type (%s) or float32, both of one type, got %s" % (dtype, t.dtype))
         if t.device != x.device:
             raise _lib.PgnnError("layer_norm: rows on %s, gains on %s" % (x.device, t.device))
         if not t.is_contiguous():
             raise _lib.PgnnError("layer_norm: contiguous gains only")
-    dim = 1
-    for k in shape:
-        dim *= k
-    if dim == 0:
-        raise ValueError("layer_norm: nothing to normalise over in %s" % (shape,))
-    if torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)):
-        return LayerNormReLU.apply(x, gamma, beta, dim, float(ln.eps), int(bool(relu)))
-    with _on_device(x.device):
-        return _layer_norm_fwd(x, gamma, beta, dim, float(ln.eps), int(bool(relu)), False)[0]
+    relu = 1 if relu else 0
+    grad = torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad))
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return LayerNormReLU.apply(x, gamma, beta, dim, ln.eps, relu) if grad else _layer_norm_fwd(x, gamma, beta, dim, ln.eps, relu, False)[0]
+    if grad:
+        return LayerNormReLU.apply(x, gamma, beta, dim, ln.eps, relu)
+    return _layer_norm_fwd(x, gamma, beta, dim, ln.eps, relu, False)[0]
 
 
 def norm(x, module, relu=False, drop_p=0.0):
