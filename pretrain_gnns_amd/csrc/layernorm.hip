@@ -50,6 +50,19 @@ __device__ __forceinline__ void load_cols(const T* __restrict__ row, int c, int 
   }
 }
 
+// the same as the 16 bytes that they are in memory (a row that is fetched ahead waits in this form)
+template <typename T>
+__device__ __forceinline__ typename Pack<T>::type load_pack(const T* __restrict__ row, int c, int dim) {
+  typename Pack<T>::type p;
+  if (c + Pack<T>::n <= dim) {
+    p = *reinterpret_cast<const typename Pack<T>::type*>(row + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < Pack<T>::n; ++e) p[e] = c + e < dim ? row[c + e] : (T)0.f;
+  }
+  return p;
+}
+
 template <typename T, int VE>
 __device__ __forceinline__ void store_cols(T* __restrict__ row, int c, int dim, const float (&v)[VE]) {
   if (c + VE <= dim) {
@@ -121,11 +134,22 @@ __global__ void __launch_bounds__(kBlock) k_layer_norm_fwd(const T* __restrict__
     load_gain<W, VE>(beta, (lane + LPR * q) * VE, dim, 0.f, b[q]);
   }
   // whole workgroups iterate together when a row is shared by all of it (the barrier in row_sum); lane groups of 16 and 64 do not meet
-  for (int64_t r = (int64_t)blockIdx.x * G + threadIdx.x / LPR; r < rows; r += (int64_t)gridDim.x * G) {
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t r = (int64_t)blockIdx.x * G + threadIdx.x / LPR;
+  typename Pack<T>::type ahead[NV];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int q = 0; q < NV; ++q) ahead[q] = load_pack<T>(x + row * ldx, (lane + LPR * q) * VE, dim);
+  };
+  if (r < rows) fetch(r);
+  for (; r < rows; r += step) {
     float v[NV][VE];
     float s[1] = {0.f};
 #pragma unroll
-    for (int q = 0; q < NV; ++q) load_cols<T, VE>(x + r * ldx, (lane + LPR * q) * VE, dim, v[q]);
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[q][e] = (float)ahead[q][e];
+    if (r + step < rows) fetch(r + step);
 #pragma unroll
     for (int q = 0; q < NV; ++q)
 #pragma unroll
@@ -177,14 +201,32 @@ __global__ void __launch_bounds__(kBlock) k_layer_norm_bwd(const T* __restrict__
 #pragma unroll
     for (int e = 0; e < VE; ++e) dw[q][e] = db[q][e] = 0.f;
   }
-  for (int64_t r = (int64_t)blockIdx.x * G + threadIdx.x / LPR; r < rows; r += (int64_t)gridDim.x * G) {
-    float v[NV][VE], g[NV][VE];
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t r = (int64_t)blockIdx.x * G + threadIdx.x / LPR;
+  // the next row is on its way while this one is summed: a row's round trip through its sums is longer than its memory latency
+  typename Pack<T>::type px[NV], pg[NV];
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto fetch = [&](int64_t row) {
+    next_mean = save_mean[row];
+    next_rstd = save_rstd[row];
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-      load_cols<T, VE>(x + r * ldx, (lane + LPR * q) * VE, dim, v[q]);
-      load_cols<T, VE>(dy + r * lddy, (lane + LPR * q) * VE, dim, g[q]);
+      px[q] = load_pack<T>(x + row * ldx, (lane + LPR * q) * VE, dim);
+      pg[q] = load_pack<T>(dy + row * lddy, (lane + LPR * q) * VE, dim);
     }
-    const float mean = save_mean[r], rstd = save_rstd[r];
+  };
+  if (r < rows) fetch(r);
+  for (; r < rows; r += step) {
+    float v[NV][VE], g[NV][VE];
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        v[q][e] = (float)px[q][e];
+        g[q][e] = (float)pg[q][e];
+      }
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < rows) fetch(r + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
