@@ -416,13 +416,21 @@ __global__ void __launch_bounds__(1024) k_layer_norm_gain_final(const float* __r
   }
 }
 
-// lanes per row: the fewest whose registers hold it (at most 32 values each)
-inline int lanes_per_row(int64_t dim) { return dim <= 16 * 32 ? 16 : dim <= 64 * 32 ? 64 : 256; }
+// lanes per row: the fewest that hold it with fewer than 32 values each -- with 32 the backward's registers leave one wave per SIMD
+// (2048 fp32: 104 us on 64 lanes, 90 on 256; 512 bf16: 57 on 16, 48 on 64; but 448 fp32, 28 values: 98 on 16, 110 on 64; 1500 bf16, 24
+// values: 55 on 64, 95 on 256; 40 M values each)
+inline int lanes_per_row(int64_t dim, int per_vector) {
+  const int64_t most = 31 / per_vector * per_vector;
+  return dim <= 16 * most ? 16 : dim <= 64 * most ? 64 : 256;
+}
 
-// workgroups of the backward: enough rows in flight to cover HBM's latency, few enough partials
+// workgroups of the backward: two per CU cover HBM's latency and leave few partials; beyond 4096 columns the registers of a workgroup fill
+// a CU and the partials are as large as rows, so one (4882 x 8192 fp32 118 us with 512, 111 with 256, bf16 84 and 65; 9765 x 4096 fp32 98
+// and 111).  Rows of a wave or more: at least two per lane group, for the partials' sake (2048 x 1500 bf16 17.1 us with one, 14.1 with two;
+// 2048 x 256 on 16 lanes 7.5 with one, 9.6 with two)
 inline int64_t bwd_blocks(int64_t rows, int64_t dim) {
-  const int64_t groups = dim > kRegDim ? 1 : kBlock / lanes_per_row(dim);
-  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, groups), 2 * 256));
+  const int64_t groups = dim > kRegDim ? 1 : kBlock / lanes_per_row(dim, 4);  // (of fp32 rows; 16-bit rows may have fewer)
+  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, groups == 16 ? groups : 2 * groups), dim > 4096 ? 256 : 512));
 }
 
 struct FwdArgs {
@@ -463,7 +471,7 @@ void by_vectors(int nv, const Args& a) {
 template <typename T, typename W, typename Args>
 void by_width(const Args& a) {
   constexpr int VE = Pack<T>::n, MAXNV = 32 / VE;
-  const int lpr = lanes_per_row(a.dim), nv = (int)ceil_div(a.dim, lpr * VE);
+  const int lpr = lanes_per_row(a.dim, VE), nv = (int)ceil_div(a.dim, lpr * VE);
   if (lpr == 16) by_vectors<T, W, 16, MAXNV>(nv, a);
   else if (lpr == 64) by_vectors<T, W, 64, MAXNV>(nv, a);
   else by_vectors<T, W, 256, MAXNV>(nv, a);

@@ -68,7 +68,7 @@ def test_newton_schulz_refusals():
     lib = _lib.load()
     R, C, n = _arrays([(300, 600), (0, 7), (5, 4)])
     need = lib.pgnn_newton_schulz_workspace_bytes(R, C, n)
-    assert need >= 4 * (300 * 640 + 2 * 600 * 320 + 2 * 300 * 320)  # X, X^T twice, A, B
+    assert need >= 4 * (2 * 600 * 320 + 2 * 300 * 320)  # X^T twice, A, B
     many = _arrays([(64, 64)] * 1000)
     assert lib.pgnn_newton_schulz_workspace_bytes(*many) < 60 * 100 * 1024  # taken in chunks
     for bad in ([(32769, 1)], [(1, 32769)], [(-1, 4)]):
