@@ -14,7 +14,8 @@
 // doubled what the last product writes and reads: ten 300 x 600 14.0 instead of 12.5 us).  A and B are symmetric: only the tiles on
 // and above the diagonal are computed, and written twice.  a X is added behind the product B X, in fp32: as a I inside B it would stand in
 // the middle of each long sum and cost the small terms their last bits (4096 x 4096: 6.5e-6 of the 64-bit result instead of 3e-6).
-// All matrices of a call share each launch: 2 + 3 steps launches whatever their number.
+// All matrices of a call share each launch: 2 + 2 steps launches if all are small (kSmall), 2 + 3 steps if none is, one if all are tiny
+// (k_ns_tiny).  The launches stand in stream order and use nothing of an earlier call's workspace.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -27,7 +28,7 @@ namespace {
 
 constexpr int kMaxJobs = 48;         // matrices per launch (the job table travels in the kernel arguments: 3.4 KB at most)
 constexpr int kMaxSteps = 32;
-constexpr int kMaxParts = 256;       // partial sums of squares per matrix
+constexpr int kMaxParts = 1024;      // partial sums of squares per matrix (256: one wave per SIMD, 4096 x 4096 40 us)
 constexpr int64_t kNormPart = 4096;  // elements per partial sum, at least
 constexpr int64_t kChunkBytes = 2ll << 30;  // a call's matrices are taken in chunks of at most this much workspace
 constexpr int kBK = 32;              // contraction per stage: one MFMA
@@ -43,7 +44,8 @@ __host__ __device__ inline int parts_of(int64_t k, int64_t n) {
 // where a matrix's planes are in its part of the workspace (bytes): the exponents and the partial sums in front, at fixed places; planes
 // of 64 k columns are multiples of 256 bytes by themselves
 constexpr int kExpRow = kMaxSteps + 1;  // exponents of X_t, A_t, B_t, Z_t: four rows
-constexpr int64_t kExps = 0, kParts = 768, kPlanes = kParts + kMaxParts * 8;
+constexpr int kMaxSplit = 128;          // tiles of a launch that are formed in parts, at most (a ticket each)
+constexpr int64_t kExps = 0, kParts = 768, kTickets = kParts + kMaxParts * 8, kPlanes = kTickets + kMaxSplit * 4;
 static_assert(4 * kExpRow * 4 <= kParts && kPlanes % 256 == 0, "");
 // A matrix on planes lies in blocks of 16 rows x 32 columns, the high plane's 1 KB and then the low one's, down a column of blocks and then
 // the next (what a stage of a product takes of an operand is one piece).  Inside a block the lane (fr, fc) of a wave that takes it as an operand -- row fr, columns 8 fc .. 8 fc + 7 -- has the 16
@@ -79,13 +81,16 @@ __device__ __forceinline__ void piece_of(int p, int& r, int& c) {
   c = block % (WIDE / 32) * 32 + fc * 8;
 }
 
-// a matrix of the call: its first workgroup in this launch, its sizes (k <= n), whether G has more rows than columns, its workspace
+// a matrix of a launch: its first workgroup, its sizes (k <= n), whether G has more rows than columns, which matrix of the call it is, its
+// workspace
 struct Job {
   int first, k, n, tall;
   int64_t off;
+  int64_t slot;
 };
 struct Jobs {
   int count, blocks, xcds;
+  int split, parts;  // of a product: the first `split` tiles are formed in `parts` parts (1: none)
   char* ws;
   Job job[kMaxJobs];
 };
@@ -114,13 +119,12 @@ struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps
 
 // the job of a workgroup: every lane loads one, a ballot finds the last that begins at or before this workgroup, its fields are read from
 // that lane.  One round trip to the kernel arguments; a bisection and a load of what it found are five
-struct Found : Job { int index; };
-__device__ __forceinline__ Found find_job(const Jobs& jobs, int b) {
+__device__ __forceinline__ Job find_job(const Jobs& jobs, int b) {
   const int lane = threadIdx.x & 63;
   const Job mine = jobs.job[min(lane, kMaxJobs - 1)];
   const int at = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(lane < jobs.count && mine.first <= b)) - 1);
-  Found f;
-  f.index = at;
+  Job f;
+  f.slot = __builtin_amdgcn_readlane((int)mine.slot, at);
   f.first = __builtin_amdgcn_readlane(mine.first, at);
   f.k = __builtin_amdgcn_readlane(mine.k, at);
   f.n = __builtin_amdgcn_readlane(mine.n, at);
@@ -132,13 +136,13 @@ __device__ __forceinline__ Found find_job(const Jobs& jobs, int b) {
 // 16 bytes of G at the element's own alignment
 template <typename T> struct Piece { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); static constexpr int n = 16 / sizeof(T); };
 
-// partial sums of squares in float64 (millions of terms, squares of gradients far below 1); Muon: the momentum is advanced here
+// one of 256 threads' share of partial sum `part` of the squares, in float64 (millions of terms, squares of gradients far below 1); Muon:
+// the momentum is advanced here
 template <typename T, bool MUON>
-__global__ void __launch_bounds__(256) k_ns_norm(Jobs jobs, Sources from, Muon<MUON> mu) {
-  const Found job = find_job(jobs, blockIdx.x);
-  const int j = job.index;
+__device__ __forceinline__ double squares(const Job& job, int part, int thread, const Sources& from, const Muon<MUON>& mu) {
+  const int j = (int)job.slot;
   const int rows = job.tall ? job.n : job.k, cols = job.tall ? job.k : job.n;
-  const int nparts = parts_of(job.k, job.n), part = blockIdx.x - job.first;
+  const int nparts = parts_of(job.k, job.n);
   const T* g = static_cast<const T*>(from.src[j]);
   const int64_t ld = from.ld[j];
   constexpr int E = Piece<T>::n;
@@ -153,40 +157,62 @@ __global__ void __launch_bounds__(256) k_ns_norm(Jobs jobs, Sources from, Muon<M
   // a dense matrix is one long row; else the workgroup's lanes walk the pieces of row after row
   const bool dense = ld == cols || rows == 1;
   const int64_t width = dense ? (int64_t)rows * cols : cols, pieces = (width + E - 1) / E;
-  const int64_t stride = (int64_t)nparts * 256, start = (int64_t)part * 256 + threadIdx.x;
+  const int64_t stride = (int64_t)nparts * 256, start = (int64_t)part * 256 + thread;
   int64_t r = 0, c = start;
   if (!dense) { r = start / pieces; c = start - r * pieces; }
   const int64_t dr = dense ? 0 : stride / pieces, dc = dense ? stride : stride - dr * pieces;
-  while (dense ? c < pieces : r < rows) {
-    const int64_t at = r * ld + c * E;
-    [[maybe_unused]] float* m = nullptr;
-    if constexpr (MUON) m = mu.momentum[j] + at;  // (dense: ld == cols)
-    if (c * E + E <= width) {
-      const typename Piece<T>::type p = *reinterpret_cast<const typename Piece<T>::type*>(g + at);
-      typename Piece<float>::type mv = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (MUON) mv = *reinterpret_cast<typename Piece<float>::type*>(m);
+  const int64_t nrows = dense ? 1 : rows;
+  while (c < pieces && r < nrows) {
+    // four pieces on their way at a time; what is no whole piece is added on the spot
+    typename Piece<T>::type p[4];
+    [[maybe_unused]] typename Piece<float>::type mv[4];
+    int64_t at[4];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float t = mv[e & 3];
-        add((float)p[e], t);
-        mv[e & 3] = t;
-      }
-      if constexpr (MUON) *reinterpret_cast<typename Piece<float>::type*>(m) = mv;
-    } else {
-      for (int e = 0; e < E && c * E + e < width; ++e) {
-        float t = 0.f;
-        if constexpr (MUON) t = m[e];
-        add((float)g[at + e], t);
-        if constexpr (MUON) m[e] = t;
+    for (int q = 0; q < 4; ++q) {
+      at[q] = -1;
+      if (c < pieces && r < nrows) {
+        const int64_t a = r * ld + c * E;
+        if (c * E + E <= width) {
+          at[q] = a;
+          p[q] = *reinterpret_cast<const typename Piece<T>::type*>(g + a);
+          if constexpr (MUON) mv[q] = *reinterpret_cast<const typename Piece<float>::type*>(mu.momentum[j] + a);
+        } else {
+          for (int e = 0; e < E && c * E + e < width; ++e) {
+            float m = 0.f;
+            if constexpr (MUON) m = mu.momentum[j][a + e];  // (Muon: dense, ld == cols)
+            add((float)g[a + e], m);
+            if constexpr (MUON) mu.momentum[j][a + e] = m;
+          }
+        }
+        c += dc;
+        r += dr;
+        if (!dense && c >= pieces) { c -= pieces; ++r; }
       }
     }
-    c += dc;
-    r += dr;
-    if (!dense && c >= pieces) { c -= pieces; ++r; }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (at[q] >= 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float m = 0.f;
+          if constexpr (MUON) m = mv[q][e & 3];
+          add((float)p[q][e], m);
+          if constexpr (MUON) mv[q][e & 3] = m;
+        }
+        if constexpr (MUON) *reinterpret_cast<typename Piece<float>::type*>(mu.momentum[j] + at[q]) = mv[q];
+      }
   }
-  __shared__ double lds[4];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  return s;  // (of the wave)
+}
+
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(256) k_ns_norm(Jobs jobs, Sources from, Muon<MUON> mu) {
+  const Job job = find_job(jobs, blockIdx.x);
+  const int part = blockIdx.x - job.first;
+  __shared__ double lds[4];
+  const double s = squares<T, MUON>(job, part, threadIdx.x, from, mu);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0)
@@ -204,12 +230,32 @@ __device__ __forceinline__ void split8(const float (&v)[8], f16x8& h, f16x8& l) 
   l = __builtin_bit_cast(f16x8, make_uint4(ll[0], ll[1], ll[2], ll[3]));
 }
 
+// the bound on X_0 from the norm, and what a step makes of a bound: exponents of A, B, Z and the next X
+__device__ __forceinline__ float first_bound(const Bounds& bd, double norm) {
+  float u = (float)(norm / (norm + (double)bd.eps)) * 1.001f;
+  if (!(u >= 0x1p-60f)) u = 0x1p-60f;  // (also a NaN: everything becomes NaN whatever the scale)
+  return u <= bd.cap_x[0] ? u : bd.cap_x[0];
+}
+struct StepExps { int a, b, z, y; };
+__device__ __forceinline__ StepExps step_bounds(const Bounds& bd, int t, float& u) {
+  const float a = fabsf(bd.coef[t][0]), b = fabsf(bd.coef[t][1]), c = fabsf(bd.coef[t][2]);
+  StepExps e;
+  const float al = fmaxf(1.001f * u * u, 0x1p-60f);
+  e.a = plane_exponent(al);
+  const float be = fmaxf(fminf(1.001f * al * (b + al * c), bd.cap_b[t]), 0x1p-60f);
+  e.b = plane_exponent(be);
+  e.z = plane_exponent(fmaxf(1.001f * u * (b + al * c), 0x1p-60f));  // Z = b X + c A X
+  u = fmaxf(fminf((a + be) * u, bd.cap_x[t + 1]), 0x1p-60f);
+  e.y = plane_exponent(u);
+  return e;
+}
+
 // X_0^T as planes, and the exponents of all planes to come
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<MUON> mu, Bounds bd) {
   const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
-  const Found job = find_job(jobs, b);
-  const int j = job.index;
+  const Job job = find_job(jobs, b);
+  const int j = (int)job.slot;
   const bool tall = job.tall;
   const int rows = tall ? job.n : job.k, cols = tall ? job.k : job.n;
   const Layout l = layout_of(job.k, job.n);
@@ -217,30 +263,27 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
   __shared__ float tile[64][65];
   __shared__ double red[4];
   const int nparts = parts_of(job.k, job.n);
-  double s = (int)threadIdx.x < nparts ? reinterpret_cast<const double*>(base + kParts)[threadIdx.x] : 0.0;
+  double s = 0.0;
+  for (int q = threadIdx.x; q < nparts; q += 256) s += reinterpret_cast<const double*>(base + kParts)[q];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
   const float inv = (float)(1.0 / (norm + (double)bd.eps));
-  float u = (float)(norm / (norm + (double)bd.eps)) * 1.001f;
-  if (!(u >= 0x1p-60f)) u = 0x1p-60f;  // (also a NaN: everything becomes NaN whatever the scale)
-  if (!(u <= bd.cap_x[0])) u = bd.cap_x[0];
+  float u = first_bound(bd, norm);
   const int e0 = plane_exponent(u);
   const int local = b - job.first;
+  if (local == 0 && threadIdx.x < kMaxSplit) reinterpret_cast<unsigned*>(base + kTickets)[threadIdx.x] = 0;
   if (local == 0 && threadIdx.x == 0) {
     int* e = reinterpret_cast<int*>(base + kExps);
     e[0] = e0;
     for (int t = 0; t < bd.steps; ++t) {
-      const float a = fabsf(bd.coef[t][0]), b = fabsf(bd.coef[t][1]), c = fabsf(bd.coef[t][2]);
-      const float al = fmaxf(1.001f * u * u, 0x1p-60f);
-      e[kExpRow + t] = plane_exponent(al);                                                       // A
-      const float be = fmaxf(fminf(1.001f * al * (b + al * c), bd.cap_b[t]), 0x1p-60f);
-      e[2 * kExpRow + t] = plane_exponent(be);                                                 // B
-      e[3 * kExpRow + t] = plane_exponent(fmaxf(1.001f * u * (b + al * c), 0x1p-60f));          // Z = b X + c A X
-      u = fmaxf(fminf((a + be) * u, bd.cap_x[t + 1]), 0x1p-60f);
-      e[t + 1] = plane_exponent(u);                                                                    // X
+      const StepExps x = step_bounds(bd, t, u);
+      e[kExpRow + t] = x.a;
+      e[2 * kExpRow + t] = x.b;
+      e[3 * kExpRow + t] = x.z;
+      e[t + 1] = x.y;
     }
   }
   const int tc = (int)((cols + 63) / 64), r0 = local / tc * 64, c0 = local % tc * 64;
@@ -353,18 +396,20 @@ __device__ __forceinline__ void read_turned(const uint32_t (&at)[4], f16x8 (&hi)
   }
 }
 
-// One TT x TT tile of a product on planes, C[i][j] = sum_l P(i, l) Q(j, l).  Four waves of TT/2 x TT/2; two fetch P and two fetch Q by LDS
-// DMA, STAGES - 1 stages ahead.  A stage is 32 deep: of A A and B X, where l runs along the operands' rows, a column of TT/16 blocks of
+// One TT x TT tile of a product on planes, C[i][j] = sum_l P(i, l) Q(j, l).  G groups, each with every G-th stage, of four waves of TT/2 x
+// TT/2; two fetch P and two fetch Q by LDS DMA, STAGES - 1 of the group's stages ahead.  A stage is 32 deep: of A A and B X, where l runs along the operands' rows, a column of TT/16 blocks of
 // each; of X X^T, where l runs down the rows of X^T, two rows of TT/32 blocks, whose fragments (8 l of one column per lane) are two
 // ds_read_b64_tr_b16 each: a 16-lane group hands over 4 rows x 16 columns turned.
-template <int TT, int STAGES, int PHASE, typename TO, bool MUON>
-__global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
+template <int TT, int STAGES, int G, int PHASE, typename TO, bool MUON>
+__global__ void __launch_bounds__(256 * G) k_ns_product(Jobs jobs, Last<PHASE> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
   constexpr int MI = TT / 32, OPER = TT * kBK * 4, STAGE = 2 * OPER, NJ = TT / 16;
   constexpr int LDT = TT + 4;  // floats per row of the epilogue's tile: 16-byte rows, neighbours four banks apart
   extern __shared__ __align__(16) char smem[];
-  const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
-  const Found job = find_job(jobs, b);
-  const int j = job.index;
+  const int in_parts = jobs.split * jobs.parts;  // workgroups of them, in front
+  const bool split = (int)blockIdx.x < in_parts;
+  const int b = split ? (int)blockIdx.x / jobs.parts : jobs.split + xcd_remap(blockIdx.x - in_parts, jobs.blocks - in_parts, jobs.xcds);
+  const Job job = find_job(jobs, b);
+  const int j = (int)job.slot;
   const int k = job.k, n = job.n;
   const Layout l = layout_of(k, n);
   char* base = jobs.ws + job.off;
@@ -374,7 +419,7 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
   const int eX = exps[step], eA = exps[kExpRow + step], eB = exps[2 * kExpRow + step], eY = exps[step + 1];
   const int64_t xt_in = step & 1 ? l.xt1 : l.xt0, xt_out = step & 1 ? l.xt0 : l.xt1;
   const _Float16* XT = reinterpret_cast<const _Float16*>(base + xt_in);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = (threadIdx.x >> 6) & 3, lane = threadIdx.x & 63;
   const int i0 = ti * TT, j0 = tj * TT, ldk = (int)l.ldk;
 
   // the wave's DMA pieces: 1 KB each, NJ of its half of P (waves 0, 1) or Q (waves 2, 3)
@@ -403,27 +448,36 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
     }
   }
   auto issue = [&](int t) {
-    char* dst = smem + (t % STAGES) * STAGE + wave * (OPER / 2);
+    if (t * G + group >= nk) return;
+    char* dst = smem + (t % STAGES * G + group) * STAGE + wave * (OPER / 2);
 #pragma unroll
     for (int q = 0; q < NJ; ++q)
-      __builtin_amdgcn_global_load_lds(PGNN_GPTR(src + (size_t)offs[q] + (size_t)t * advance), PGNN_LPTR(dst + q * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(PGNN_GPTR(src + (size_t)offs[q] + (size_t)(t * G + group) * advance), PGNN_LPTR(dst + q * 1024), 16, 0, 0);
   };
 
   // the epilogue's operand (A behind A A, X^T behind B X) at this thread's pieces of the tile, fetched in front of everything else: its
   // round trip to memory hides behind the product
-  constexpr int MINE = TT * TT / 8 / 256;  // pieces of eight columns per thread
+  constexpr int MINE = TT * TT / 8 / (256 * G);  // pieces of eight columns per thread
   const int out_rows = PHASE <= kPoly ? ldk : (int)l.rows;
   [[maybe_unused]] f16x8 eh[MINE], el[MINE];
-  if constexpr (PHASE != kGram) {
+  [[maybe_unused]] auto fetch_operand = [&]() {
     const _Float16* E = PHASE == kPoly ? reinterpret_cast<const _Float16*>(base + l.a) : XT;
 #pragma unroll
     for (int q = 0; q < MINE; ++q) {
       int r, c;
-      piece_of<TT>(q * 256 + threadIdx.x, r, c);
+      piece_of<TT>(q * 256 * G + threadIdx.x, r, c);
       const int64_t at = piece_at(out_rows, min(j0 + r, out_rows - 1), min(i0 + c, ldk - 8));
       eh[q] = *reinterpret_cast<const f16x8*>(E + at);
       el[q] = *reinterpret_cast<const f16x8*>(E + at + kBlockHalfs / 2);
     }
+  };
+  if constexpr (PHASE != kGram) {
+    if (!split) fetch_operand();
+  }
+  if (split) {  // this workgroup's share of the contraction
+    const int part = blockIdx.x % jobs.parts, k0 = (int)((int64_t)nk * part / jobs.parts);
+    nk = (int)((int64_t)nk * (part + 1) / jobs.parts) - k0;
+    src += k0 * advance;
   }
 
   const int wi = (wave >> 1) * (TT / 2), wj = (wave & 1) * (TT / 2);
@@ -453,17 +507,17 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
     for (int c = 0; c < MI; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 
 #pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t)
-    if (t < nk) issue(t);
-  for (int t = 0; t < nk; ++t) {
+  for (int t = 0; t < STAGES - 1; ++t) issue(t);
+  for (int t = 0; t * G < nk; ++t) {
     // stage t has landed; behind the barrier every wave's part of it has, and every wave is done with the buffer refilled below
-    if (t + STAGES - 2 < nk) gemm_wait_vmcnt_imm<(STAGES - 2) * NJ>();
+    if ((t + STAGES - 2) * G + group < nk) gemm_wait_vmcnt_imm<(STAGES - 2) * NJ>();
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (t + STAGES - 1 < nk) issue(t + STAGES - 1);
-    const char* st = smem + (t % STAGES) * STAGE;
+    issue(t + STAGES - 1);
+    if (G > 1 && t * G + group >= nk) break;  // (an odd number of stages: the last round is the first group's; no barrier follows in the loop)
+    const char* st = smem + (t % STAGES * G + group) * STAGE;
     f16x8 ph[MI], pl[MI], qh[MI], ql[MI];
     if constexpr (PHASE == kGram) {
       const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)st;
@@ -498,6 +552,63 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
     asm volatile("" ::: "memory");
   }
 
+  // the second group's sums to the first, through LDS
+  if constexpr (G > 1) {
+    __syncthreads();
+    f32x4* hand = reinterpret_cast<f32x4*>(smem) + (threadIdx.x & 255);
+    if (group) {
+#pragma unroll
+      for (int e = 0; e < MI * MI; ++e) hand[e * 256] = acc[e / MI][e % MI];
+    }
+    __syncthreads();
+    if (!group) {
+#pragma unroll
+      for (int e = 0; e < MI * MI; ++e) acc[e / MI][e % MI] += hand[e * 256];
+    }
+  }
+
+  // a tile in parts: each part's sums go to memory that the launch does not use otherwise (the X^T to come, behind B X what was A), and
+  // the part that arrives last adds all of them up in their own order and goes on as if it had formed the whole tile
+  if (split) {
+    uint64_t* mem = reinterpret_cast<uint64_t*>(base + (PHASE <= kPoly ? xt_out : l.a)) + (int64_t)(b - job.first) * jobs.parts * (TT * TT / 2) + (threadIdx.x & 255);
+    uint64_t* mine = mem + (int64_t)(blockIdx.x % jobs.parts) * (TT * TT / 2);
+    if (!group) {
+#pragma unroll
+      for (int e = 0; e < MI * MI; ++e) {
+        const uint4 w = __builtin_bit_cast(uint4, acc[e / MI][e % MI]);
+        publish(mine + e * 512, (uint64_t)w.y << 32 | w.x);
+        publish(mine + e * 512 + 256, (uint64_t)w.w << 32 | w.z);
+      }
+      publish_commit();
+    }
+    __syncthreads();
+    unsigned* ticket = reinterpret_cast<unsigned*>(base + kTickets) + (b - job.first);
+    if (threadIdx.x == 0) {
+      const bool last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)jobs.parts - 1u;
+      if (last) publish(ticket, 0u);
+      *reinterpret_cast<int*>(smem) = last;
+    }
+    __syncthreads();
+    if (!*reinterpret_cast<int*>(smem)) return;
+    asm volatile("" ::: "memory");
+    for (int part = 0; part < jobs.parts && !group; ++part) {
+      const uint64_t* from_part = mem + (int64_t)part * (TT * TT / 2);
+      uint64_t w[MI * MI][2];
+#pragma unroll
+      for (int e = 0; e < MI * MI; ++e) {
+        w[e][0] = fetch_published(from_part + e * 512);
+        w[e][1] = fetch_published(from_part + e * 512 + 256);
+      }
+#pragma unroll
+      for (int e = 0; e < MI * MI; ++e) {
+        const f32x4 v = __builtin_bit_cast(f32x4, make_uint4((uint32_t)w[e][0], (uint32_t)(w[e][0] >> 32), (uint32_t)w[e][1], (uint32_t)(w[e][1] >> 32)));
+        f32x4& sum = acc[e / MI][e % MI];
+        sum = part == 0 ? v : sum + v;
+      }
+    }
+    if constexpr (PHASE != kGram) fetch_operand();
+  }
+
   // epilogue: the tile to LDS as fp32 [j][i] (a lane holds four consecutive i of one j), out row by row as the operand lies (rows j),
   // and once more turned (rows i) where the mirror image of a symmetric tile or a wide G wants it
   __syncthreads();
@@ -505,11 +616,13 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
   const float f = PHASE == kGram ? ldexpf(1.f, eA - 2 * eX) : PHASE == kPoly ? ldexpf(cc, eB - 2 * eA)
                 : PHASE == kApply ? ldexpf(1.f, eY - eX - eB) : ldexpf(1.f, -eX - eB);
   const float fe = PHASE == kPoly ? ldexpf(cb, eB - eA) : PHASE == kApply ? ldexpf(ca, eY - eX) : ldexpf(ca, -eX);
+  if (!group) {
 #pragma unroll
-  for (int a = 0; a < MI; ++a)
+    for (int a = 0; a < MI; ++a)
 #pragma unroll
-    for (int c = 0; c < MI; ++c)
-      *reinterpret_cast<f32x4*>(tile + (wj + c * 16 + fr) * LDT + wi + a * 16 + fc * 4) = acc[a][c] * f;
+      for (int c = 0; c < MI; ++c)
+        *reinterpret_cast<f32x4*>(tile + (wj + c * 16 + fr) * LDT + wi + a * 16 + fc * 4) = acc[a][c] * f;
+  }
   __syncthreads();
 
   auto planes_out = [&](_Float16* d, int r, int c, const float (&v)[8]) {
@@ -546,7 +659,7 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
 #pragma unroll
   for (int q = 0; q < MINE; ++q) {
     int r, c;
-    piece_of<TT>(q * 256 + threadIdx.x, r, c);
+    piece_of<TT>(q * 256 * G + threadIdx.x, r, c);
     float* p = tile + r * LDT + c;
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
     float v[8];
@@ -576,7 +689,7 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
 #pragma unroll
   for (int q = 0; q < MINE; ++q) {
     int r, c;
-    piece_of<TT>(q * 256 + threadIdx.x, r, c);
+    piece_of<TT>(q * 256 * G + threadIdx.x, r, c);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[(c + e) * LDT + r];
@@ -594,18 +707,20 @@ __global__ void __launch_bounds__(256) k_ns_product(Jobs jobs, Last<PHASE> to, M
 
 // The second half of a step for small k in one launch: X <- a X + A Z, Z = b X + c A X, a strip of 32 rows of X^T per workgroup (one row of
 // X^T knows nothing of another, so the two products need no exchange between workgroups; B = b A + c A A would, and one more launch).  It
-// costs 4 k^2 n instead of 2 k^3 + 2 k^2 n operations, which a small matrix has to spare: its launches are bound by their latency.
+// costs 4 k^2 n instead of 2 k^3 + 2 k^2 n operations, which a small matrix has to spare: its launches are bound by their latency.  k <=
+// kSmall takes it (against B and B X; us for the whole iteration: 100 x 200 75 and 97, ten 300 x 600 147 and 157, forty 391 and 373, ten
+// 384 x 768 190 and 198, twenty-four 403 and 324, 512 x 512 179 and 157).
 // The strip and Z lie in LDS, A streams from L2 straight into registers -- every wave
 // takes whole 16-row blocks of A, so nothing of A is read twice by a workgroup -- RING pairs of 32-deep steps ahead; the strip's
 // fragments of a pair are read from LDS while the pair before it multiplies.  A lane's four results
 // are four consecutive columns of one row of X^T: they go to LDS as they are, and the strip leaves in whole rows.
-constexpr int kStrip = 32, kSmall = 512;  // kSmall: two strips in 128 KB of LDS
+constexpr int kStrip = 32, kSmall = 320;
 
 template <int RING, bool LAST, typename TO, bool MUON>
 __global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast : kApply> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
   extern __shared__ __align__(16) char smem[];
   const int b = xcd_remap(blockIdx.x, jobs.blocks, jobs.xcds);
-  const Found job = find_job(jobs, b);
+  const Job job = find_job(jobs, b);
   const int k = job.k, n = job.n;
   const Layout l = layout_of(k, n);
   char* base = jobs.ws + job.off;
@@ -736,11 +851,11 @@ __global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast :
         put(strip, r, i, v);  // nobody else reads these four any more
       } else if (j0 + r < n) {
         const int64_t at = job.tall ? (int64_t)(j0 + r) * k + i : (int64_t)i * n + j0 + r, next = job.tall ? 1 : n;
-        TO* d = static_cast<TO*>(to.dst[job.index]) + at;
+        TO* d = static_cast<TO*>(to.dst[job.slot]) + at;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (i + e >= k) break;
-          if constexpr (MUON) d[e * next] = fmaf(-mu.rate[job.index], v[e], d[e * next] * mu.keep);
+          if constexpr (MUON) d[e * next] = fmaf(-mu.rate[job.slot], v[e], d[e * next] * mu.keep);
           else d[e * next] = (TO)v[e];
         }
       }
@@ -754,6 +869,204 @@ __global__ void __launch_bounds__(512) k_ns_apply(Jobs jobs, Last<LAST ? kLast :
       d[(int64_t)(q >> 8) * down * (kBlockHalfs / 8) + (q & 255)] = reinterpret_cast<const f16x8*>(strip)[q];
   }
 }
+
+// The whole iteration of one small matrix (k <= kTinyK, n <= kTinyN) in one workgroup, X^T, A and Z in LDS: no launch but this one.  Gram:
+// waves 0-3 and 4-7 each form A's 64 x 64 over every other 32 rows of X^T, the second four hand theirs over through LDS.  Then a wave takes
+// whole 16-row blocks of X^T, whose new rows depend on nothing but themselves and A: Z = b X + c A X into scratch of its own, X <- a X + A Z
+// back in place, no barrier between.  Every sum is taken in the order of the kernels above where a launch of theirs is small.
+constexpr int kTinyK = 64, kTinyN = 384;
+
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(512) k_ns_tiny(Jobs jobs, Sources from, Results to, Muon<MUON> mu, Bounds bd) {
+  extern __shared__ __align__(16) char smem[];  // (alone: read_turned flips bit 6 of its addresses, so LDS begins with the blocks)
+  const Job job = jobs.job[blockIdx.x];
+  const int j = (int)job.slot;
+  const int k = job.k, n = job.n, np = (n + 31) & ~31, down = np / 16;
+  const bool tall = job.tall;
+  const int rows = tall ? n : k, cols = tall ? k : n;
+  char* const xt = smem;                  // blocks [2][down][planes]
+  char* const am = smem + np * 256;       // blocks [2][4][planes]
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, fr = lane & 15, fc = lane >> 4;
+  char* const zed = am + 16384 + wave * 4096;  // blocks [2][planes], of this wave alone
+  double* const red = reinterpret_cast<double*>(am);
+  const T* g = static_cast<const T*>(from.src[j]);
+  const int64_t ld = from.ld[j];
+
+  // eight elements of the thread on their way at a time; row of element e by a multiplication (e cols < 2^32 / cols: exact)
+  const uint32_t magic = (uint32_t)((0xffffffffull + cols) / cols);
+  const int total = rows * cols;
+  auto row_of = [&](int e) { return cols == 1 ? e : (int)__umulhi((uint32_t)e, magic); };
+  auto load8 = [&](int e0, float (&v)[8], float (&m)[8]) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int e = min(e0 + 512 * q, total - 1), r = row_of(e);
+      v[q] = (float)g[r * ld + (e - r * cols)];
+      if constexpr (MUON) m[q] = mu.momentum[j][e];
+    }
+  };
+  // the norm by the same sums as k_ns_norm and k_ns_split: waves 0-3 and 4-7 take a part each
+  const int nparts = parts_of(k, n);
+  for (int part = wave >> 2; part < nparts; part += 2) {
+    const double s = squares<T, MUON>(job, part, threadIdx.x & 255, from, mu);
+    if (lane == 0) red[part * 4 + (wave & 3)] = s;
+  }
+  for (int e = threadIdx.x; e < np * 16; e += 512) reinterpret_cast<uint4*>(xt)[e] = make_uint4(0, 0, 0, 0);  // rows n .., columns k ..
+  __syncthreads();
+  double s = lane < nparts ? (red[lane * 4] + red[lane * 4 + 1]) + (red[lane * 4 + 2] + red[lane * 4 + 3]) : 0.0;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  const double norm = sqrt(s);
+  const float inv = (float)(1.0 / (norm + (double)bd.eps));
+  float u = first_bound(bd, norm);
+  int eX = plane_exponent(u);
+  const float scale = ldexpf(1.f, eX);
+  for (int e0 = threadIdx.x; e0 < total; e0 += 8 * 512) {
+    float v[8], m[8];  // (the momentum: what the workgroup has just written, behind a barrier)
+    load8(e0, v, m);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int e = e0 + 512 * q, r = row_of(e), c = e - r * cols;
+      if (e >= total) continue;
+      if constexpr (MUON) v[q] = mu.nesterov ? fmaf(mu.mu, m[q], v[q]) : m[q];
+      const float x = v[q] * inv * scale;
+      const _Float16 h = (_Float16)x;
+      _Float16* d = reinterpret_cast<_Float16*>(xt) + piece_at(np, tall ? r : c, (tall ? c : r) & ~7) + ((tall ? c : r) & 7);
+      d[0] = h;
+      d[kBlockHalfs / 2] = (_Float16)low_part(x, h);
+    }
+  }
+  __syncthreads();
+
+  const uint32_t xt_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)xt;
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  auto frag = [&](const char* block) { return *reinterpret_cast<const f16x8*>(block + unit_of(fr, fc) * 16); };
+  // four columns i .. i + 3 of row r inside a column of blocks of `d` blocks each
+  auto quad = [&](char* m, int d, int r, int i) { return m + ((i >> 5) * d + (r >> 4)) * 2048 + unit_of(r & 15, (i >> 3) & 3) * 16 + (i & 7) * 2; };
+  auto put = [&](char* at, const float (&v)[4]) {
+    uint32_t h[2], lo[2];
+    split2(v[0], v[1], h[0], lo[0]);
+    split2(v[2], v[3], h[1], lo[1]);
+    *reinterpret_cast<uint2*>(at) = make_uint2(h[0], h[1]);
+    *reinterpret_cast<uint2*>(at + 1024) = make_uint2(lo[0], lo[1]);
+  };
+  // acc[a] = (rows 16 a .. of A) . (16 rows of op)^T; op's blocks: column of blocks h at op + h * stride
+  auto by_a = [&](const char* op, int stride, f32x4 (&acc)[4]) {
+    f32x4 cross[4];  // (the terms in the order of k_ns_apply)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) acc[a] = cross[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f16x8 oh = frag(op + h * stride), ol = frag(op + h * stride + 1024);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f16x8 ah = frag(am + (h * 4 + a) * 2048), alow = frag(am + (h * 4 + a) * 2048 + 1024);
+        cross[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, ol, cross[a], 0, 0, 0);
+        acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, oh, acc[a], 0, 0, 0);
+        cross[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(alow, oh, cross[a], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a) acc[a] += cross[a];
+  };
+  for (int t = 0; t < bd.steps; ++t) {
+    const StepExps ex = step_bounds(bd, t, u);
+    const float ca = bd.coef[t][0], cb = bd.coef[t][1], cc = bd.coef[t][2];
+    {  // A = X X^T
+      const int pb = (wave >> 1 & 1) * 2, qb = (wave & 1) * 2, half = wave >> 2;
+      f32x4 acc[2][2];
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      auto at = [&](int block) {  // row l = 8 fc + fr / 4, columns 4 (fr & 3) .. of block's 16
+        const int unit = 2 * (block & 1) + ((fr & 3) >> 1);
+        return xt_at + (uint32_t)(((block >> 1) * down + (fc >> 1)) * 2048 + unit_of(8 * (fc & 1) + (fr >> 2), unit) * 16 + (fr & 1) * 8);
+      };
+      for (int st = half; st < np / 32; st += 2) {
+        f16x8 h[4], lo[4];
+        const uint32_t o = (uint32_t)st * 4096;
+        read_turned({at(pb) + o, at(pb + 1) + o, at(qb) + o, at(qb + 1) + o}, h, lo);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            acc[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[a], lo[2 + c], acc[a][c], 0, 0, 0);
+            acc[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[a], h[2 + c], acc[a][c], 0, 0, 0);
+            acc[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[a], h[2 + c], acc[a][c], 0, 0, 0);
+          }
+      }
+      f32x4* other = reinterpret_cast<f32x4*>(am + 16384 + (wave & 3) * 4096) + lane;  // (the first four waves' scratch: idle here)
+      if (half) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) other[(a * 2 + c) * 64] = acc[a][c];
+      }
+      __syncthreads();
+      if (!half) {
+        const float f = ldexpf(1.f, ex.a - 2 * eX);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const f32x4 v = (acc[a][c] + other[(a * 2 + c) * 64]) * f;
+            put(quad(am, 4, (qb + c) * 16 + fr, (pb + a) * 16 + 4 * fc), {v[0], v[1], v[2], v[3]});
+          }
+      }
+      __syncthreads();
+    }
+    const bool last = t + 1 == bd.steps;
+    const float fz = ldexpf(cc, ex.z - ex.a - eX), fzx = ldexpf(cb, ex.z - eX);
+    const int ey = last ? 0 : ex.y;
+    const float fy = ldexpf(1.f, ey - ex.a - ex.z), fyx = ldexpf(ca, ey - eX);
+    for (int blk = wave; blk < down; blk += 8) {
+      float x[4][4];
+      f32x4 acc[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const char* q = quad(xt, down, blk * 16 + fr, a * 16 + 4 * fc);
+        const f16x4 h = *reinterpret_cast<const f16x4*>(q), lo = *reinterpret_cast<const f16x4*>(q + 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[a][e] = (float)h[e] + (float)lo[e];
+      }
+      by_a(xt + blk * 2048, down * 2048, acc);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = fmaf(fzx, x[a][e], acc[a][e] * fz);
+        put(quad(zed, 1, fr, a * 16 + 4 * fc), z);
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): Z is whole before any lane of the wave reads it
+      asm volatile("" ::: "memory");
+      by_a(zed, 2048, acc);
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(fyx, x[a][e], acc[a][e] * fy);
+        const int r = blk * 16 + fr, i = a * 16 + 4 * fc;
+        if (!last) {
+          put(quad(xt, down, r, i), v);
+        } else if (r < n) {
+          const int64_t at = tall ? (int64_t)r * k + i : (int64_t)i * n + r, next = tall ? 1 : n;
+          T* d = static_cast<T*>(to.dst[j]) + at;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < k) {
+              if constexpr (MUON) d[e * next] = fmaf(-mu.rate[j], v[e], d[e * next] * mu.keep);
+              else d[e * next] = (T)v[e];
+            }
+        }
+      }
+    }
+    eX = ex.y;
+    __syncthreads();
+  }
+}
+
+constexpr int kPartStages = 8, kMaxTileParts = 16;  // a part is at least 8 stages deep (16: 1500 x 1500 452 instead of 425 us, two 2048 x 2048 1138 instead of 1153; 4: 2048 x 2048 742 instead of 713)
 
 // max over x in [0, u] of |a x^p + b x^(p+2) + c x^(p+4)| for p = 1 and 0, by its stationary points
 double odd_max(double a, double b, double c, double u) {
@@ -814,13 +1127,39 @@ void place(Jobs& jobs, Count blocks_of) {
   }
 }
 
-template <int TT, int STAGES, int PHASE, typename TO, bool MUON>
+// A CU's matrix cores are busy with one tile, so a launch takes the time of ceil(tiles / CUs) tiles one after the other: what is left over a
+// multiple of the CUs' number is formed in as many parts as give every CU one.  They stand in front of the launch, so that their sums meet
+// while the CUs work on whole tiles.  4096 x 4096 (528 tiles of A, 16 left over on 256 CUs, in 16 parts) 4255 -> 3692 us; with two or three
+// parts to a tile the way through memory costs more than it saves beside whole tiles (ten 1024 x 2048, 104 left over: 1261 -> 1321).
+template <int TT, int PHASE>
+void split_rest(Jobs& jobs) {
+  const int rest = jobs.blocks % num_cu();
+  jobs.split = 0;
+  jobs.parts = 1;
+  if (rest == 0 || rest > kMaxSplit) return;
+  int64_t parts = std::min(num_cu() / rest, kMaxTileParts);
+  for (int j = 0; j < jobs.count && jobs.job[j].first < rest; ++j) {
+    const Job& q = jobs.job[j];
+    const Layout l = layout_of(q.k, q.n);
+    const int tiles = std::min(rest, j + 1 < jobs.count ? jobs.job[j + 1].first : jobs.blocks) - q.first;
+    if (tiles == 0) continue;
+    const int64_t room = 4 * l.ldk * (PHASE <= kPoly ? l.rows : l.ldk), stages = (PHASE == kGram ? q.n : q.k) / kBK;
+    parts = std::min(std::min(parts, room / ((int64_t)tiles * TT * TT * 4)), stages / kPartStages);
+  }
+  if (parts < (rest == jobs.blocks ? 2 : 4)) return;
+  jobs.split = rest;
+  jobs.parts = (int)parts;
+  jobs.blocks += rest * (jobs.parts - 1);
+}
+
+template <int TT, int STAGES, int G, int PHASE, typename TO, bool MUON>
 void launch_product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
   place(jobs, [](const Job& q) { return tiles_of<TT>(q.k, q.n, PHASE <= kPoly); });
-  constexpr size_t lds = std::max<size_t>((size_t)STAGES * 4 * TT * kBK * 2, (size_t)TT * (TT + 4) * 4);
-  const void* fn = (const void*)k_ns_product<TT, STAGES, PHASE, TO, MUON>;
+  split_rest<TT, PHASE>(jobs);
+  constexpr size_t lds = std::max<size_t>((size_t)STAGES * G * 2 * TT * kBK * 4, (size_t)TT * (TT + 4) * 4);
+  const void* fn = (const void*)k_ns_product<TT, STAGES, G, PHASE, TO, MUON>;
   allow_big_lds(fn, lds);
-  hipLaunchKernelGGL((k_ns_product<TT, STAGES, PHASE, TO, MUON>), dim3(jobs.blocks), dim3(256), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
+  hipLaunchKernelGGL((k_ns_product<TT, STAGES, G, PHASE, TO, MUON>), dim3(jobs.blocks), dim3(256 * G), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
 }
 
 template <int RING, bool LAST, typename TO, bool MUON>
@@ -831,46 +1170,69 @@ void launch_apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<
   allow_big_lds((const void*)k_ns_apply<RING, LAST, TO, MUON>, lds);
   hipLaunchKernelGGL((k_ns_apply<RING, LAST, TO, MUON>), dim3(jobs.blocks), dim3(64 * waves), lds, st, jobs, to, mu, step, c[0], c[1], c[2]);
 }
-
-template <int TT, int STAGES, typename TO, bool MUON>
-void run_steps(Jobs& jobs, const Results& to, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
-  const Nothing no{0};
+template <bool LAST, typename TO, bool MUON>
+void apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
   int most = 0;
-  int64_t strips = 0;
+  for (int j = 0; j < jobs.count; ++j) most = std::max(most, jobs.job[j].k);
+  if (most <= 128) launch_apply<2, LAST, TO, MUON>(jobs, to, mu, step, c, most, st);  // a wave has two pairs of steps in all
+  else launch_apply<4, LAST, TO, MUON>(jobs, to, mu, step, c, most, st);
+}
+
+// Tiles of 128 where they give every CU one (a launch with 256, 320 or 384 of them 61, 49 and 49 us, with tiles of 64 66, 52 and 57; with
+// 136 55 instead of 43), else of 64.  Where those do not give every CU more than one, a tile's stages go to two groups of four waves in turn:
+// alone on its SIMD a wave waits for the barrier, LDS and the matrix cores one after the other (300 x 600 11.6 -> 10.4 us, 1024 x 1024
+// 15.2 -> 12.7, 1000 x 4096 46 -> 36 a launch; eight stages in flight instead of four changed nothing).
+template <int PHASE, typename TO, bool MUON>
+void product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
+  int64_t big = 0, small = 0;
   for (int j = 0; j < jobs.count; ++j) {
-    most = std::max(most, jobs.job[j].k);
-    strips += ceil_div(jobs.job[j].n, kStrip);
+    big += tiles_of<128>(jobs.job[j].k, jobs.job[j].n, PHASE <= kPoly);
+    small += tiles_of<64>(jobs.job[j].k, jobs.job[j].n, PHASE <= kPoly);
   }
-  const bool small = most <= kSmall && strips <= num_cu();
-  for (int t = 0; t < bd.steps; ++t) {
-    launch_product<TT, STAGES, kGram, float, false>(jobs, no, no, t, bd.coef[t], st);
-    if (small) {
-      // (k <= 128: a wave has two pairs of steps in all)
-      if (t + 1 < bd.steps) {
-        if (most <= 128) launch_apply<2, false, float, false>(jobs, no, no, t, bd.coef[t], most, st);
-        else launch_apply<4, false, float, false>(jobs, no, no, t, bd.coef[t], most, st);
-      } else {
-        if (most <= 128) launch_apply<2, true, TO, MUON>(jobs, to, mu, t, bd.coef[t], most, st);
-        else launch_apply<4, true, TO, MUON>(jobs, to, mu, t, bd.coef[t], most, st);
-      }
-      continue;
-    }
-    launch_product<TT, STAGES, kPoly, float, false>(jobs, no, no, t, bd.coef[t], st);
-    if (t + 1 < bd.steps) launch_product<TT, STAGES, kApply, float, false>(jobs, no, no, t, bd.coef[t], st);
-    else launch_product<TT, STAGES, kLast, TO, MUON>(jobs, to, mu, t, bd.coef[t], st);
-  }
+  if (big >= num_cu()) launch_product<128, 2, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
+  else if (small > num_cu()) launch_product<64, 4, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
+  else launch_product<64, 4, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
 }
 
 template <typename T, bool MUON>
 void run_chunk(Jobs& jobs, const Sources& from, const Results& to, const Muon<MUON>& mu, const Bounds& bd, hipStream_t st) {
+  const Nothing no{0};
+  // k_ns_tiny where every matrix of the chunk fits it: beside others in the list its launch would only stand in their way (the list of a
+  // 5-layer network, with 3 x 300 among 300 x 600: 153 us without it, 194 with it), and there the small ones cost next to nothing
+  int tiny_n = 0;
+  for (int j = 0; j < jobs.count && tiny_n >= 0; ++j)
+    tiny_n = jobs.job[j].k <= kTinyK && jobs.job[j].n <= kTinyN ? std::max(tiny_n, jobs.job[j].n) : -1;
+  if (tiny_n > 0) {
+    const size_t lds = (size_t)((tiny_n + 31) & ~31) * 256 + 16384 + 8 * 4096;
+    allow_big_lds((const void*)k_ns_tiny<T, MUON>, lds);
+    hipLaunchKernelGGL((k_ns_tiny<T, MUON>), dim3(jobs.count), dim3(512), lds, st, jobs, from, to, mu, bd);
+    return;
+  }
+  Jobs few{}, many{};
+  few.ws = many.ws = jobs.ws;
+  few.xcds = many.xcds = jobs.xcds;
+  for (int j = 0; j < jobs.count; ++j) {
+    Jobs& half = jobs.job[j].k <= kSmall ? few : many;
+    half.job[half.count++] = jobs.job[j];
+  }
   place(jobs, [](const Job& q) { return parts_of(q.k, q.n); });
   hipLaunchKernelGGL((k_ns_norm<T, MUON>), dim3(jobs.blocks), dim3(256), 0, st, jobs, from, mu);
   place(jobs, [](const Job& q) { return tiles_of<64>(q.k, q.n, false); });
   hipLaunchKernelGGL((k_ns_split<T, MUON>), dim3(jobs.blocks), dim3(256), 0, st, jobs, from, mu, bd);
-  int64_t big = 0;
-  for (int j = 0; j < jobs.count; ++j) big += tiles_of<128>(jobs.job[j].k, jobs.job[j].n, true);
-  if (big >= num_cu()) run_steps<128, 2, T, MUON>(jobs, to, mu, bd, st);
-  else run_steps<64, 4, T, MUON>(jobs, to, mu, bd, st);
+  for (int t = 0; t < bd.steps; ++t) {
+    const bool last = t + 1 == bd.steps;
+    const float* c = bd.coef[t];
+    product<kGram, float, false>(jobs, no, no, t, c, st);
+    if (few.count) {
+      if (last) apply<true, T, MUON>(few, to, mu, t, c, st);
+      else apply<false, float, false>(few, no, no, t, c, st);
+    }
+    if (many.count) {
+      product<kPoly, float, false>(many, no, no, t, c, st);
+      if (last) product<kLast, T, MUON>(many, to, mu, t, c, st);
+      else product<kApply, float, false>(many, no, no, t, c, st);
+    }
+  }
 }
 
 // the matrices [from, to) of a chunk: at most kMaxJobs, and kChunkBytes unless one alone takes more
@@ -927,7 +1289,7 @@ int run_all(const char* what, const int64_t* rows, const int64_t* cols, int64_t 
     for (int64_t j = from; j < to; ++j) {
       if (rows[j] == 0 || cols[j] == 0) continue;
       const int q = jobs.count++;
-      jobs.job[q] = Job{0, (int)std::min(rows[j], cols[j]), (int)std::max(rows[j], cols[j]), rows[j] > cols[j], off};
+      jobs.job[q] = Job{0, (int)std::min(rows[j], cols[j]), (int)std::max(rows[j], cols[j]), rows[j] > cols[j], off, q};
       off += layout_of(jobs.job[q].k, jobs.job[q].n).bytes;
       fill.set(src, res, mu, q, j);
     }
