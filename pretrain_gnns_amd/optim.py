@@ -207,7 +207,7 @@ class Muon:
         self._flat = torch.zeros(total, dtype=torch.float32, device=self._own[0].device)
         self.state = {p: {"momentum_buffer": self._flat[o:o + p.numel()].view(p.shape)} for p, o in zip(self._own, offs)}
         self.param_groups = [{"params": self._own, "lr": lr, "weight_decay": weight_decay, "momentum": momentum, "nesterov": nesterov}]
-        self._table, self._table_key = None, None
+        self._sizes, self._tables = None, None  # of the live parameters: their sizes, and what follows from sizes alone
 
     def zero_grad(self, set_to_none=True):
         _zero_grads(self._own, set_to_none)
@@ -223,23 +223,23 @@ class Muon:
         live = [p for p in self._own if p.grad is not None and p.numel()]
         if not live:
             return
-        lib = load()
-        key = tuple([p.data_ptr() for p in live] + [p.grad.data_ptr() for p in live])
-        if key != self._table_key:  # the tables are built again only when a pointer moved
-            for p in live:
-                if p.grad.dtype != torch.float32 or not p.grad.is_contiguous() or p.grad.device != p.device:
-                    raise _lib.PgnnError("pretrain_gnns_amd.optim.Muon: gradients must be contiguous fp32 on the parameter's device")
-            n = len(live)
-            pointers = lambda ts: (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])
-            rows, cols = (ctypes.c_int64 * n)(*[p.size(0) for p in live]), (ctypes.c_int64 * n)(*[p.size(1) for p in live])
-            self._table = (pointers(live), pointers([p.grad for p in live]), pointers([self.state[p]["momentum_buffer"] for p in live]), rows, cols, n,
-                           lib.pgnn_newton_schulz_workspace_bytes(rows, cols, n), [self._scale(p) for p in live])
-            self._table_key = key
-        P, G, M, rows, cols, n, need, scales = self._table
+        lib, n, dev = load(), len(live), live[0].device
+        grads, momenta = [p.grad for p in live], [self.state[p]["momentum_buffer"] for p in live]
+        for kind, tensors in (("parameters", live), ("gradients", grads), ("momentum buffers", momenta)):
+            for t, p in zip(tensors, live):
+                if t.dtype is not torch.float32 or t.device != dev or t.shape != p.shape or not t.is_contiguous():
+                    raise _lib.PgnnError("pretrain_gnns_amd.optim.Muon: %s must be contiguous fp32 of the parameter's size and on its device" % kind)
+        sizes = [p.shape for p in live]
+        if sizes != self._sizes:
+            rows, cols = (ctypes.c_int64 * n)(*[r for r, _ in sizes]), (ctypes.c_int64 * n)(*[c for _, c in sizes])
+            self._tables = rows, cols, lib.pgnn_newton_schulz_workspace_bytes(rows, cols, n), [self._scale(p) for p in live]
+            self._sizes = sizes
+        rows, cols, need, scales = self._tables
+        P, G, M = ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (live, grads, momenta))
         group = self.param_groups[0]
         lr = float(group["lr"])
-        with _on_device(live[0].device):
-            ws = _call_workspace(need, live[0].device)
+        with _on_device(dev):
+            ws = _call_workspace(need, dev)
             check(lib.pgnn_muon_step(P, G, M, (ctypes.c_float * n)(*[lr * s for s in scales]), rows, cols, n, float(group["momentum"]),
                                      int(bool(group["nesterov"])), 1.0 - lr * float(group["weight_decay"]), self._coef, self.ns_steps, self.eps,
                                      ws.data_ptr(), ws.numel(), stream_ptr()), "pgnn_muon_step")

@@ -348,6 +348,28 @@ def test_muon_refusals():
     assert w.grad is None
 
 
+def test_muon_looks_at_every_steps_tensors():
+    """another gradient at the address of the last one, another momentum buffer"""
+    from pretrain_gnns_amd import _lib, optim
+    w = _params([(6, 6)])[0]
+    opt = optim.Muon([w])
+    w.grad = _matrix(6, 6).to(DEV)
+    opt.step()
+    before = w.detach().clone()
+    w.grad = w.grad.t()  # same address
+    with pytest.raises(_lib.PgnnError, match="contiguous fp32"):
+        opt.step()
+    w.grad = w.grad.t()
+    for bad in (torch.zeros(6, 5, device=DEV), torch.zeros(6, 6, device=DEV, dtype=torch.float16), torch.zeros(6, 6)):
+        opt.state[w]["momentum_buffer"] = bad
+        with pytest.raises(_lib.PgnnError, match="momentum buffers"):
+            opt.step()
+    assert torch.equal(w, before)
+    opt.state[w]["momentum_buffer"] = torch.zeros(6, 6, device=DEV)
+    opt.step()
+    assert not torch.equal(w, before)
+
+
 def test_training_step_with_layer_norm_and_muon():
     """the masking step of a network with LayerNorms, its weights under Muon and the rest under Adam: the update is the definition's, from
     the gradients that the step left"""
