@@ -394,11 +394,13 @@ int pgnn_adam_step(float* const* params, const float* const* grads, const int64_
  *   X = G / (|G|_F + eps), transposed while rows > cols; per step t, with (a, b, c) = coefficients[3 t .. 3 t + 2] (host, fp32):
  *   A = X X^T, X <- a X + (b A + c A A) X;  result = X, dense [rows, cols] of the same `type` (PGNN_F32 / PGNN_BF16 / PGNN_F16), rounded once
  * with the error of fp32 products throughout.  dst[j] may be src[j].  1 to 32 steps; coefficients under which the bound on X's singular
- * values (they start in [0, 1]) passes 2^20 are refused.  A matrix of zeros gives zeros, one with a NaN or an infinity gives NaN throughout.
+ * values (they start in [0, 1]) passes 2^20 are refused.  A matrix of zeros gives zeros (eps > 0), one with a NaN or an infinity NaN throughout;
+ * what is left of values of X that start below 2^-60 (a norm far below eps) is lost.
  * The same workspace serves both calls; matrices are taken in chunks (at most 48, and 2 GiB of workspace unless one needs more).
  * pgnn_muon_step: fp32, dense; per matrix  M <- mu M + G;  U = nesterov ? G + mu M : M;  p <- keep p - rates[j] orthogonal(U)
- * (keep = 1 - lr weight_decay; rates: host).  No allocation, no atomics, bitwise reproducible; may be captured in a graph (rates, mu and
- * keep are then the captured ones).
+ * (keep = 1 - lr weight_decay; rates: host).  No allocation; the same call gives the same bits (how a long sum is cut depends on all
+ * matrices of the call and on the number of compute units); may be captured in a graph (rates, mu and keep are then the captured ones).
+ * Concurrent calls need a workspace each; its contents are of no use afterwards.
  * ------------------------------------------------------------------------------------------ */
 size_t pgnn_newton_schulz_workspace_bytes(const int64_t* rows, const int64_t* cols, int64_t count);
 int pgnn_newton_schulz(const void* const* src, const int64_t* ld_src, void* const* dst, const int64_t* rows, const int64_t* cols, int64_t count,

@@ -230,6 +230,16 @@ __device__ __forceinline__ void split8(const float (&v)[8], f16x8& h, f16x8& l) 
   l = __builtin_bit_cast(f16x8, make_uint4(ll[0], ll[1], ll[2], ll[3]));
 }
 
+// 1 / (norm + eps) as a factor in [0.5, 1) and an exponent: as one fp32 number it would leave the normal range for norms beyond 2^126
+__device__ __forceinline__ float inverse(double norm, float eps, int& e) { return (float)frexp(1.0 / (norm + (double)eps), &e); }
+
+// v inv 2^shift.  By the power first: v may be subnormal.  Rounded here in every kernel (not fused with what follows)
+__device__ __forceinline__ float scaled(float v, int shift, float inv) {
+  float x = ldexpf(v, shift) * inv;
+  asm("" : "+v"(x));
+  return x;
+}
+
 // the bound on X_0 from the norm, and what a step makes of a bound: exponents of A, B, Z and the next X
 __device__ __forceinline__ float first_bound(const Bounds& bd, double norm) {
   float u = (float)(norm / (norm + (double)bd.eps)) * 1.001f;
@@ -270,9 +280,11 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
-  const float inv = (float)(1.0 / (norm + (double)bd.eps));
+  int shift;
+  const float inv = inverse(norm, bd.eps, shift);
   float u = first_bound(bd, norm);
   const int e0 = plane_exponent(u);
+  shift += e0;
   const int local = b - job.first;
   if (local == 0 && threadIdx.x < kMaxSplit) reinterpret_cast<unsigned*>(base + kTickets)[threadIdx.x] = 0;
   if (local == 0 && threadIdx.x == 0) {
@@ -287,7 +299,6 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
     }
   }
   const int tc = (int)((cols + 63) / 64), r0 = local / tc * 64, c0 = local % tc * 64;
-  const float scale = ldexpf(1.f, e0);
   const T* g = static_cast<const T*>(from.src[j]);
   const int64_t ld = from.ld[j];
   constexpr int E = Piece<T>::n, ACROSS = 64 / E;
@@ -319,7 +330,7 @@ __global__ void __launch_bounds__(256) k_ns_split(Jobs jobs, Sources from, Muon<
       }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) tile[r][c + e] = v[e] * inv * scale;
+    for (int e = 0; e < E; ++e) tile[r][c + e] = scaled(v[e], shift, inv);
   }
   __syncthreads();
   _Float16* d = reinterpret_cast<_Float16*>(base + l.xt0);
@@ -916,10 +927,11 @@ __global__ void __launch_bounds__(512) k_ns_tiny(Jobs jobs, Sources from, Result
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
   const double norm = sqrt(s);
-  const float inv = (float)(1.0 / (norm + (double)bd.eps));
+  int shift;
+  const float inv = inverse(norm, bd.eps, shift);
   float u = first_bound(bd, norm);
   int eX = plane_exponent(u);
-  const float scale = ldexpf(1.f, eX);
+  shift += eX;
   for (int e0 = threadIdx.x; e0 < total; e0 += 8 * 512) {
     float v[8], m[8];  // (the momentum: what the workgroup has just written, behind a barrier)
     load8(e0, v, m);
@@ -928,7 +940,7 @@ __global__ void __launch_bounds__(512) k_ns_tiny(Jobs jobs, Sources from, Result
       const int e = e0 + 512 * q, r = row_of(e), c = e - r * cols;
       if (e >= total) continue;
       if constexpr (MUON) v[q] = mu.nesterov ? fmaf(mu.mu, m[q], v[q]) : m[q];
-      const float x = v[q] * inv * scale;
+      const float x = scaled(v[q], shift, inv);
       const _Float16 h = (_Float16)x;
       _Float16* d = reinterpret_cast<_Float16*>(xt) + piece_at(np, tall ? r : c, (tall ? c : r) & ~7) + ((tall ? c : r) & 7);
       d[0] = h;

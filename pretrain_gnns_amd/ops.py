@@ -1943,8 +1943,8 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     """orthogonalise matrices: ``steps`` Newton-Schulz products X <- a X + (b X X^T + c (X X^T)^2) X from X = G / (|G|_F + eps), which take
     every singular value towards 1 and leave the singular vectors alone (csrc/newton_schulz.hip).  ``g``: a tensor [..., rows, cols] of
     fp32, bf16 or fp16, or a list of such matrices of any sizes (one type and device): all of them share the launches.  Returns new
-    contiguous tensors of the same type, computed with the error of fp32 products whatever the type and rounded once.  No gradient flows
-    through it (it makes updates, not activations)."""
+    contiguous tensors of the same type, computed with the error of fp32 products whatever the type and rounded once; the same call gives
+    the same bits.  No gradient flows through it (it makes updates, not activations)."""
     import ctypes
     several = isinstance(g, (list, tuple))
     tensors = list(g) if several else [g]

@@ -157,6 +157,90 @@ def test_newton_schulz_of_any_size_of_gradient(scale):
             assert rel < 2.0 ** -16, rel  # 5 steps that each lose 2^-22 and magnify what was lost by up to 3.9, to first order: in quadrature < 64 * 2^-22
 
 
+@pytest.mark.parametrize("shape", [(20, 30), (90, 65)])
+def test_newton_schulz_at_the_ends_of_the_types_range(shape):
+    """a norm beyond fp32's largest number, whose inverse is below its smallest; subnormal values with eps = 0"""
+    ops = _ops()
+    for g, kw in ((_matrix(*shape).div(_matrix(*shape).abs().max()) * 3.3e38, {}), (_matrix(*shape) * 2.0 ** -140, {"eps": 0.0})):
+        out = ops.newton_schulz(g.to(DEV), **kw)
+        want = _iterate(g.double(), **kw)
+        rel = ((out.cpu().double() - want).norm() / want.norm()).item()
+        assert rel < 2.0 ** -16, rel  # (as in the test above)
+
+
+# one tile more or one row more than a rule's limit: the one-launch form (64 x 384), the strips (320), and tiles that are formed in parts
+# because they are few (700 x 650)
+@pytest.mark.parametrize("rows,cols", [(64, 384), (385, 64), (65, 384), (320, 321), (321, 320), (384, 20), (700, 650), (520, 1030)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_newton_schulz_at_the_limits_of_its_rules(rows, cols, dtype):
+    ops = _ops()
+    g = _matrix(rows, cols).to(dtype)
+    d = g.to(DEV)
+    out = ops.newton_schulz(d)
+    _compare(out, g)
+    assert torch.equal(out, ops.newton_schulz(d))
+
+
+@pytest.mark.parametrize("count,rows,cols,look", [(13, 330, 1100, (0, 5, 12)), (8, 1024, 1030, (0, 7)), (5, 1030, 900, (0, 4))])
+def test_newton_schulz_left_over_tiles(count, rows, cols, look):
+    """a few tiles more than compute units, in a graph as well: the parts' tickets are clear again behind every call"""
+    ops = _ops()
+    base = _matrix(rows, cols)
+    gen = torch.Generator().manual_seed(5)
+    g = torch.stack([base[torch.randperm(rows, generator=gen)] for _ in range(count)])  # (each matrix another one)
+    d = g.to(DEV)
+    out = ops.newton_schulz(d)
+    for i in look:
+        _compare(out[i], g[i])
+    assert torch.equal(out, ops.newton_schulz(d))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ops.newton_schulz(d)
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+        eager = ops.newton_schulz(d)
+        torch.cuda.synchronize()
+        assert torch.equal(again, out) and torch.equal(eager, out)
+
+
+def test_newton_schulz_two_streams_at_once():
+    """calls that overlap on two streams: each has its own workspace"""
+    ops = _ops()
+    a, b = _matrix(700, 650).to(DEV), _matrix(600, 800, 1).to(DEV)
+    want = ops.newton_schulz(a), ops.newton_schulz(b)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(8):
+        for s, m in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                outs.append(ops.newton_schulz(m))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i & 1]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("shape", [(30, 40), (300, 100), (400, 500)])
+def test_newton_schulz_in_place_at_the_c_entry(shape):
+    import ctypes
+    from pretrain_gnns_amd import _lib
+    ops = _ops()
+    for dtype in (torch.float32, torch.bfloat16):
+        g = _matrix(*shape).to(dtype).to(DEV)
+        want = ops.newton_schulz(g)
+        lib = _lib.load()
+        one = lambda v: (ctypes.c_int64 * 1)(v)
+        R, C = one(shape[0]), one(shape[1])
+        ws = torch.empty(lib.pgnn_newton_schulz_workspace_bytes(R, C, 1), dtype=torch.uint8, device=DEV)
+        ptr = (ctypes.c_void_p * 1)(g.data_ptr())
+        coef = (ctypes.c_float * 15)(*(COEF * 5))
+        code = {torch.float32: 0, torch.bfloat16: 1}[dtype]
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.pgnn_newton_schulz(ptr, C, ptr, R, C, 1, code, coef, 5, 1e-7, ws.data_ptr(), ws.numel() - 1, stream) != 0  # too small
+        assert lib.pgnn_newton_schulz(ptr, C, ptr, R, C, 1, code, coef, 5, 1e-7, ws.data_ptr(), ws.numel(), stream) == 0
+        assert torch.equal(g, want)
+
+
 def test_newton_schulz_zeros_and_bad_values():
     ops = _ops()
     z = torch.zeros(70, 90, device=DEV)
@@ -290,6 +374,25 @@ def test_muon_steps(kw):
         assert ((m.cpu().double() - ref.m[i]).abs() <= 4 * 2.0 ** -24 * 4 * ref.m[i].abs().max()).all()
         off = (p.detach().cpu().double() - ref.p[i]).abs()
         assert (off <= ref.slack[i]).all(), (i, (off / ref.slack[i]).max().item())
+
+
+@pytest.mark.parametrize("shapes", [[(3, 300), (64, 384), (1, 1)], [(6, 300), (300, 600), (400, 350), (119, 300), (1, 5)]])
+def test_muon_lists_of_one_and_of_all_sizes(shapes):
+    """a list that one launch takes, and one in which every kernel has a share"""
+    from pretrain_gnns_amd import optim
+    params = _params(shapes)
+    opt = optim.Muon(params, lr=0.02)
+    ref = _Oracle(params, lr=0.02)
+    for t in range(3):
+        grads = [_matrix(*p.shape, seed=t).to(DEV) for p in params]
+        for p, g in zip(params, grads):
+            p.grad = g
+        opt.step()
+        ref.step(grads)
+    for i, p in enumerate(params):
+        off = (p.detach().cpu().double() - ref.p[i]).abs()
+        # the fp32 momentum differs from the oracle's in its last bit, and a direction magnifies that like any rounding of its input
+        assert (off <= 2 * ref.slack[i]).all(), (i, (off / ref.slack[i]).max().item())
 
 
 def test_muon_in_a_captured_step():
