@@ -1190,10 +1190,12 @@ void apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<MUON>& 
   else launch_apply<4, LAST, TO, MUON>(jobs, to, mu, step, c, most, st);
 }
 
-// Tiles of 128 where they give every CU one (a launch with 256, 320 or 384 of them 61, 49 and 49 us, with tiles of 64 66, 52 and 57; with
-// 136 55 instead of 43), else of 64.  Where those do not give every CU more than one, a tile's stages go to two groups of four waves in turn:
-// alone on its SIMD a wave waits for the barrier, LDS and the matrix cores one after the other (300 x 600 11.6 -> 10.4 us, 1024 x 1024
-// 15.2 -> 12.7, 1000 x 4096 46 -> 36 a launch; eight stages in flight instead of four changed nothing).
+// Tiles of 128 where at least three CUs of five get one, else of 64: a launch of 162, 182 or 256 of them takes 33.8, 39.7 and 60.9 us, with
+// tiles of 64 36.1, 42.8 and 66; 78 or 136 of them 35.5 and 47.9 instead of 26.0 and 46.5.  Where the tiles do not give a CU more than one,
+// a tile's stages go to two groups of four waves in turn: alone on its SIMD a wave waits for the barrier, LDS and the matrix cores one after
+// the other (tiles of 64: 300 x 600 11.6 -> 10.4 us, 1024 x 1024 15.2 -> 12.7, 1000 x 4096 46 -> 36 a launch, eight stages in flight instead
+// of four changed nothing; of 128: 2048 x 2048 69.7 -> 60.9).  With two tiles on a CU these do that for each other: ten 1024 x 2048 134 us
+// with one group, 154 with two.
 template <int PHASE, typename TO, bool MUON>
 void product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
   int64_t big = 0, small = 0;
@@ -1201,7 +1203,8 @@ void product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, 
     big += tiles_of<128>(jobs.job[j].k, jobs.job[j].n, PHASE <= kPoly);
     small += tiles_of<64>(jobs.job[j].k, jobs.job[j].n, PHASE <= kPoly);
   }
-  if (big >= num_cu()) launch_product<128, 2, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
+  if (big > num_cu()) launch_product<128, 2, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
+  else if (5 * big >= 3 * num_cu()) launch_product<128, 2, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
   else if (small > num_cu()) launch_product<64, 4, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
   else launch_product<64, 4, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
 }
