@@ -14,8 +14,8 @@
 // doubled what the last product writes and reads: ten 300 x 600 14.0 instead of 12.5 us).  A and B are symmetric: only the tiles on
 // and above the diagonal are computed, and written twice.  a X is added behind the product B X, in fp32: as a I inside B it would stand in
 // the middle of each long sum and cost the small terms their last bits (4096 x 4096: 6.5e-6 of the 64-bit result instead of 3e-6).
-// All matrices of a call share each launch: 2 + 2 steps launches if all are small (kSmall), 2 + 3 steps if none is, one if all are tiny
-// (k_ns_tiny).  The launches stand in stream order and use nothing of an earlier call's workspace.
+// The matrices of a call share the launches: one if all are tiny (k_ns_tiny), 2 + 2 steps if all are small (kSmall), else 2 + 3 steps, and
+// `steps` more where small ones go apart from large ones.  The launches stand in stream order and use nothing of an earlier call's workspace.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1223,11 +1223,17 @@ void run_chunk(Jobs& jobs, const Sources& from, const Results& to, const Muon<MU
     hipLaunchKernelGGL((k_ns_tiny<T, MUON>), dim3(jobs.count), dim3(512), lds, st, jobs, from, to, mu, bd);
     return;
   }
+  // few: by k_ns_apply.  Beside larger ones whose tiles leave CUs idle the small ones ride along in their launches instead (five 300 x 300
+  // and five 400 x 400 224 -> 153 us); a launch that is full already is better off without them (2048 x 2048 and 119 x 2048 708, together 873)
+  int64_t larger = 0;
+  for (int j = 0; j < jobs.count; ++j)
+    if (jobs.job[j].k > kSmall) larger += tiles_of<128>(jobs.job[j].k, jobs.job[j].n, false);
+  const bool together = larger > 0 && larger < num_cu();
   Jobs few{}, many{};
   few.ws = many.ws = jobs.ws;
   few.xcds = many.xcds = jobs.xcds;
   for (int j = 0; j < jobs.count; ++j) {
-    Jobs& half = jobs.job[j].k <= kSmall ? few : many;
+    Jobs& half = jobs.job[j].k <= kSmall && !together ? few : many;
     half.job[half.count++] = jobs.job[j];
   }
   place(jobs, [](const Job& q) { return parts_of(q.k, q.n); });
