@@ -870,7 +870,8 @@ def layer_norm(x, ln, relu=False):
     """apply a ``torch.nn.LayerNorm`` module's parameters with the HIP kernels, ``relu`` fuses max(., 0) behind it.  The rows are fp32,
     bf16 or fp16 of any width and stride; the gains are of the rows' type or fp32 (mixed precision), or absent.  Statistics are per
     row, so unlike ``batch_norm`` it takes a single row and couples no data-parallel ranks.  Gradients for x, weight and bias, added
-    up in a fixed order."""
+    up in a fixed order.  To capture a backward pass, drop eager results of the same parameters first (torch ties a parameter's gradient
+    node to the stream of the result that still holds it)."""
     gamma, beta = ln.weight, ln.bias
     require_cuda(x, gamma, beta)
     shape = ln.normalized_shape

@@ -236,6 +236,35 @@ def test_layer_norm_only_what_is_asked_for():
     assert torch.equal(torch.autograd.grad(ops.layer_norm(xd, ln), xd, dy.to(DEV))[0], full[0])
 
 
+def test_layer_norm_beyond_32_bits():
+    """more than 2^31 values, dense and as rows far apart: the last rows as they come out of a small call"""
+    ops = _ops()
+    rows, dim = 2 ** 21 + 3, 1025
+    ln = _module(dim, torch.float16)
+    x = torch.zeros(rows, dim, dtype=torch.float16, device=DEV)
+    dy = torch.zeros_like(x)
+    few, dfew = _rows(8, dim, torch.float16)
+    few, dfew = few.to(DEV), dfew.to(DEV)
+    x[-8:], dy[-8:] = few, dfew
+    x.requires_grad_(True)
+    y = ops.layer_norm(x, ln)
+    got = torch.autograd.grad(y, (x, ln.weight, ln.bias), dy)
+    fl = few.clone().requires_grad_(True)
+    want_y = ops.layer_norm(fl, ln)
+    want = torch.autograd.grad(want_y, (fl, ln.weight, ln.bias), dfew)
+    assert torch.equal(y[-8:], want_y) and torch.equal(got[0][-8:], want[0])
+    assert torch.equal(y[0], ln.bias) and not got[0][:-8].any()
+    # the same eight terms however they are grouped: twice 8 half steps of fp32 of their sum, at most 8 max|dy| sqrt(dim) (|xh| <= 32.02), which
+    # is 2^-11.9 max|dy|, and two roundings to fp16
+    for a, b in zip(got[1:], want[1:]):
+        assert ((a.float() - b.float()).abs() <= torch.finfo(torch.float16).eps * b.float().abs() + 2.0 ** -11 * dfew.float().abs().max()).all()
+    del x, y, dy, got
+    wide = torch.zeros(1100, 2000003, dtype=torch.float16, device=DEV)
+    part = wide[:, 7:7 + dim]
+    part[-8:] = few
+    assert torch.equal(ops.layer_norm(part, ln)[-8:].detach(), want_y.detach())
+
+
 def test_layer_norm_streams_and_graphs():
     ops = _ops()
     ln = _module(300, torch.float32)

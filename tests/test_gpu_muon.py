@@ -204,6 +204,20 @@ def test_newton_schulz_left_over_tiles(count, rows, cols, look):
         assert torch.equal(again, out) and torch.equal(eager, out)
 
 
+def test_newton_schulz_beyond_32_bits():
+    """planes of more than 2^31 bytes, one step, against fp32 products on the device"""
+    rows, cols = 20011, 32768
+    g = torch.randn(rows, cols, device=DEV).bfloat16()
+    out = _ops().newton_schulz(g, steps=1)
+    x = g.float()
+    x *= (1 / (x.double().norm() + 1e-7)).float()
+    gram = x @ x.t()
+    b = torch.addmm(COEF[1] * gram, gram, gram, alpha=COEF[2])
+    want = torch.addmm(x, b, x, beta=COEF[0])
+    off = (out.float() - want).double().norm() / want.double().norm()
+    assert off.item() <= 2.0 ** -8 + 2.0 ** -13  # half a step of bf16 per value; the fp32 products' own error is far below the second term
+
+
 def test_newton_schulz_two_streams_at_once():
     """calls that overlap on two streams: each has its own workspace"""
     ops = _ops()
