@@ -778,9 +778,9 @@ __global__ void __launch_bounds__(256 * G) k_ns_product(Jobs jobs, Last<PHASE> t
 // The second half of a step for small k in one launch: X <- a X + A Z, Z = b X + c A X, a strip of 32 rows of X^T per workgroup (one row of
 // X^T knows nothing of another, so the two products need no exchange between workgroups; B = b A + c A A would, and one more launch).  It
 // costs 4 k^2 n instead of 2 k^3 + 2 k^2 n operations, which a small matrix has to spare: its launches are bound by their latency.  k <=
-// kSmall takes it (against B and B X; us for the whole iteration: 100 x 200 73 and 87, sixteen 128 x 2048 158 and 164, 200 x 200 94 and 99,
-// four 256 x 512 111 and 120, sixteen 256 x 1024 176 and 171, 300 x 600 124 and 118, ten of them 138 and 137, the Muon step of a 5-layer
-// network of such weights, whose heads begin another round of tiles, 145 and 158; 384 x 384 130 and 120).
+// kSmall takes it (against B and B X; us for the whole iteration: 100 x 200 73 and 87, sixteen 128 x 2048 158 and 164, 200 x
+// 200 94 and 99, four 256 x 512 111 and 120, 300 x 600 124 and 122, ten of them 136 and 137, the Muon step of a 5-layer network of such weights
+// 144.5 and 145.5; 384 x 384 130 and 118).
 // The strip and Z lie in LDS, A streams from L2 straight into registers -- every wave
 // takes whole 16-row blocks of A, so nothing of A is read twice by a workgroup -- RING pairs of 32-deep steps ahead; the strip's
 // fragments of a pair are read from LDS while the pair before it multiplies.  A lane's four results
@@ -1254,11 +1254,14 @@ void apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<MUON>& 
 
 // Tiles of 64, or of 128 from two and a half tiles of 64 per CU on: launches of 648, 675 and 1024 tiles of 64 take 36.1, 42.8 and 66 us, with
 // tiles of 128 33.8, 39.7 and 60.9; launches of 528 and 520 (300 x 600, which tiles of 128 overhang) 46.5 and 10.3, with 128 47.9 and 14.4.
-// Where the tiles do not give a CU more than one,
-// a tile's stages go to two groups of four waves in turn: alone on its SIMD a wave waits for the barrier, LDS and the matrix cores one after
-// the other (tiles of 64: 300 x 600 11.6 -> 10.4 us, 1024 x 1024 15.2 -> 12.7, 1000 x 4096 46 -> 36 a launch, eight stages in flight instead
-// of four changed nothing; of 128: 2048 x 2048 69.7 -> 60.9).  With two tiles on a CU these do that for each other: ten 1024 x 2048 134 us
-// with one group, 154 with two.
+// A wave that is alone on its SIMD waits for the barrier, LDS and the matrix cores one after the other, so a CU wants several:
+// - no more tiles than CUs: a tile's stages go to two groups of four waves in turn (tiles of 64: 300 x 600 11.6 -> 10.4 us a launch, 1000 x
+//   4096 46 -> 36; of 128: 2048 x 2048 69.7 -> 60.9).  Eight stages in flight for one group changed nothing.
+// - up to two tiles of 64 per CU: two groups each, and LDS for two tiles, i.e. two stages per group (four 700 x 800 16.0 -> 14.1, 1300 x 1300
+//   22.1 -> 21.2 against one group with four stages).
+// - more: LDS for three tiles of one group and three stages (572 and 768 tiles 21.6 -> 18.2 and 36.4 -> 31.7 against four stages, which are
+//   two tiles; 441 tiles 22.8, with two groups 21.2; two stages for five tiles: 35.0 for 768, and 32 for 476 instead of 27).
+// - tiles of 128: two of one group (ten 1024 x 2048 134 us, with two groups and thus one tile 154).
 template <int PHASE, typename TO, bool MUON>
 void product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, const float* c, hipStream_t st) {
   int64_t big = 0, small = 0;
@@ -1270,7 +1273,8 @@ void product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, 
     if (big > num_cu()) launch_product<128, 2, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
     else launch_product<128, 2, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
   }
-  else if (small > num_cu()) launch_product<64, 4, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
+  else if (small > 2 * num_cu()) launch_product<64, 3, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
+  else if (small > num_cu()) launch_product<64, 2, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
   else launch_product<64, 4, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
 }
 
