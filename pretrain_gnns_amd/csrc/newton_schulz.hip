@@ -1252,8 +1252,8 @@ void apply(Jobs& jobs, const Last<LAST ? kLast : kApply>& to, const Muon<MUON>& 
   else launch_apply<4, LAST, TO, MUON>(jobs, to, mu, step, c, most, st);
 }
 
-// Tiles of 64, or of 128 from two and a half tiles of 64 per CU on: launches of 648, 675 and 1024 tiles of 64 take 36.1, 42.8 and 66 us, with
-// tiles of 128 33.8, 39.7 and 60.9; launches of 528 and 520 (300 x 600, which tiles of 128 overhang) 46.5 and 10.3, with 128 47.9 and 14.4.
+// Tiles of 64 while three of them per CU take them all at once, else of 128: launches of 640, 648 and 675 tiles of 64 take 15.7, 28.2 and
+// 38.4 us, with tiles of 128 17.2, 31.1 and 41.9; launches of 870 and 1024 33.0 and 65.7, with tiles of 128 29.1 and 53.6.
 // A wave that is alone on its SIMD waits for the barrier, LDS and the matrix cores one after the other, so a CU wants several:
 // - no more tiles than CUs: a tile's stages go to two groups of four waves in turn (tiles of 64: 300 x 600 11.6 -> 10.4 us a launch, 1000 x
 //   4096 46 -> 36; of 128: 2048 x 2048 69.7 -> 60.9).  Eight stages in flight for one group changed nothing.
@@ -1269,7 +1269,7 @@ void product(Jobs& jobs, const Last<PHASE>& to, const Muon<MUON>& mu, int step, 
     big += tiles_of<128>(jobs.job[j].k, jobs.job[j].n, PHASE <= kPoly);
     small += tiles_of<64>(jobs.job[j].k, jobs.job[j].n, PHASE <= kPoly);
   }
-  if (2 * small >= 5 * num_cu()) {
+  if (small > 3 * num_cu()) {
     if (big > num_cu()) launch_product<128, 2, 1, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
     else launch_product<128, 2, 2, PHASE, TO, MUON>(jobs, to, mu, step, c, st);
   }
