@@ -847,7 +847,17 @@ def _layer_norm_bwd(ctx, dy):
     return dx, dgamma, dbeta, None, None, None
 
 
-_layer_norm_bwd_once = once_differentiable(_layer_norm_bwd)
+class _NoSecondDerivative(Function):
+    """gradients as they are, in a graph whose backward refuses.  (once_differentiable refuses only where the incoming gradient is part
+    of a graph itself; a constant one would leave what depends on x out without a word.)"""
+
+    @staticmethod
+    def forward(ctx, live, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("layer_norm: its gradients cannot be differentiated again")
 
 
 class LayerNormReLU(Function):
@@ -862,8 +872,11 @@ class LayerNormReLU(Function):
 
     @staticmethod
     def backward(ctx, dy):
-        # (once_differentiable's wrapper costs as much as the call: it is needed where a graph of the backward is asked for)
-        return _layer_norm_bwd_once(ctx, dy) if torch.is_grad_enabled() else _layer_norm_bwd(ctx, dy)
+        if not torch.is_grad_enabled():
+            return _layer_norm_bwd(ctx, dy)
+        with torch.no_grad():  # a graph of the backward is asked for
+            grads = _layer_norm_bwd(ctx, dy)
+        return _NoSecondDerivative.apply(torch.empty(0, device=dy.device, requires_grad=True), *grads)
 
 
 def layer_norm(x, ln, relu=False):

@@ -236,6 +236,25 @@ def test_layer_norm_only_what_is_asked_for():
     assert torch.equal(torch.autograd.grad(ops.layer_norm(xd, ln), xd, dy.to(DEV))[0], full[0])
 
 
+def test_layer_norm_has_no_second_derivative():
+    """a graph of the backward may be asked for; its use is refused, whatever the first gradient came from"""
+    ops = _ops()
+    ln = _module(30, torch.float32)
+    x, dy = _rows(5, 30, torch.float32)
+    x, dy = x.to(DEV).requires_grad_(True), dy.to(DEV)
+    want = torch.autograd.grad(ops.layer_norm(x, ln), (x, ln.weight, ln.bias), dy)
+    got = torch.autograd.grad(ops.layer_norm(x, ln), (x, ln.weight, ln.bias), dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    only, = torch.autograd.grad(ops.layer_norm(x, ln), ln.bias, dy, create_graph=True)
+    for loss in (got[0].square().sum(), got[1].sum() + x.sum(), only.sum()):
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            loss.backward()
+    y = ops.layer_norm(x, ln)
+    g, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        (y.sum() + g.sum()).backward()
+
+
 def test_layer_norm_beyond_32_bits():
     """more than 2^31 values, dense and as rows far apart: the last rows as they come out of a small call"""
     ops = _ops()
