@@ -8,7 +8,7 @@ import os
 import weakref
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -913,7 +913,9 @@ def layer_norm(x, ln, relu=False):
         if not t.is_contiguous():
             raise _lib.PgnnError("layer_norm: contiguous gains only")
     relu = 1 if relu else 0
-    grad = torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad))
+    # the tape has to see the call where gradients are recorded, and where a forward-mode tangent (which it refuses) or a trace passes through
+    grad = forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None or (
+        torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)))
     if x.device.index != torch.cuda.current_device():
         with torch.cuda.device(x.device):
             return LayerNormReLU.apply(x, gamma, beta, dim, ln.eps, relu) if grad else _layer_norm_fwd(x, gamma, beta, dim, ln.eps, relu, False)[0]

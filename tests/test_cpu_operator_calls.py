@@ -1,0 +1,63 @@
+"""CPU: the host side of the operators' calls, the launches replaced by counters (no GPU here: nothing is launched)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from pretrain_gnns_amd import ops
+
+
+class _Counting:
+    """the library as far as these tests go: workspaces of 1 KB, calls that do nothing, counted by name"""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            if name.endswith("workspace_bytes"):
+                return 1024
+            self.calls.append(name)
+            return 0
+        return call
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    """the calls' argument handling on CPU tensors"""
+    lib = _Counting()
+    monkeypatch.setattr(ops, "load", lambda: lib)
+    monkeypatch.setattr(ops, "require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(ops, "stream_ptr", lambda *index: 0)
+    monkeypatch.setattr(ops, "_ws_cache", {})
+    monkeypatch.setattr(ops, "_ws_pool", {})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return lib
+
+
+def _frozen_layer_norm(dim, **kw):
+    return torch.nn.LayerNorm(dim, **kw).requires_grad_(False)
+
+
+@pytest.mark.parametrize("kw", [{}, {"elementwise_affine": False}])
+def test_layer_norm_drops_no_forward_tangent(lib, kw):
+    """a tangent is refused as long as there is no rule for it, never dropped; a level without one changes nothing"""
+    ln, x = _frozen_layer_norm(8, **kw), torch.randn(3, 8)
+    with forward_ad.dual_level():
+        assert forward_ad.unpack_dual(ops.layer_norm(x, ln)).tangent is None
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad(), pytest.raises(NotImplementedError, match="jvp"):
+                ops.layer_norm(dual, ln)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: ops.layer_norm(t, ln), (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("kw", [{}, {"bias": False}, {"elementwise_affine": False}])
+def test_a_trace_of_layer_norm_holds_the_call(lib, kw):
+    ln, x = _frozen_layer_norm(8, **kw), torch.randn(3, 8)
+    traced = torch.jit.trace(lambda t: ops.layer_norm(t, ln, True), (x,), check_trace=False)
+    assert "LayerNormReLU" in str(traced.graph)
+    before = len(lib.calls)
+    traced(torch.randn(5, 8))
+    assert lib.calls[before:] == ["pgnn_layer_norm_fwd"]
