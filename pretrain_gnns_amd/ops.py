@@ -797,6 +797,15 @@ def _call_workspace(nbytes, device):
     return _workspace(nbytes, device)
 
 
+_PROXY_MODE = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _refuse_proxy_trace(what):
+    """make_fx records torch's own calls only: the result's memory would be in its graph, the kernel that fills it would not"""
+    if torch._C._get_dispatch_mode(_PROXY_MODE) is not None:
+        raise _lib.PgnnError("%s: make_fx cannot record it" % what)
+
+
 def _last_axis_rows(t, dim):
     """[rows, dim] view of a tensor whose trailing axes hold ``dim`` values, columns contiguous (any row stride); a copy where the
     strides allow no view"""
@@ -887,6 +896,7 @@ def layer_norm(x, ln, relu=False):
     node to the stream of the result that still holds it)."""
     gamma, beta = ln.weight, ln.bias
     require_cuda(x, gamma, beta)
+    _refuse_proxy_trace("layer_norm")
     shape = ln.normalized_shape
     if len(shape) == 1:
         dim = shape[0]
@@ -1970,6 +1980,9 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
         return []
     first = tensors[0]
     require_cuda(*tensors)
+    _refuse_proxy_trace("newton_schulz")
+    if torch._C._get_tracing_state() is not None:  # (as with make_fx: no autograd function stands for the call in the graph)
+        raise _lib.PgnnError("newton_schulz: torch.jit.trace cannot record it")
     coef = _newton_schulz_coefficients(coefficients, steps)
     src, lds, rows, cols, dst, outs, held = [], [], [], [], [], [], []
     for t in tensors:

@@ -1,9 +1,11 @@
 """CPU: the host side of the operators' calls, the launches replaced by counters (no GPU here: nothing is launched)."""
+import contextlib
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from pretrain_gnns_amd import ops
+from pretrain_gnns_amd import _lib, ops
 
 
 class _Counting:
@@ -30,6 +32,7 @@ def lib(monkeypatch):
     monkeypatch.setattr(ops, "stream_ptr", lambda *index: 0)
     monkeypatch.setattr(ops, "_ws_cache", {})
     monkeypatch.setattr(ops, "_ws_pool", {})
+    monkeypatch.setattr(ops, "_on_device", lambda device: contextlib.nullcontext())
     monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return lib
@@ -61,3 +64,18 @@ def test_a_trace_of_layer_norm_holds_the_call(lib, kw):
     before = len(lib.calls)
     traced(torch.randn(5, 8))
     assert lib.calls[before:] == ["pgnn_layer_norm_fwd"]
+
+
+def test_recorders_of_torch_calls_are_refused(lib):
+    """they would keep the result's memory and not the launch that fills it"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ln, x = _frozen_layer_norm(8), torch.randn(3, 8)
+    for op in (lambda t: ops.layer_norm(t, ln), ops.newton_schulz, lambda t: ops.newton_schulz([t, t])[1]):
+        with pytest.raises(_lib.PgnnError, match="make_fx"):
+            make_fx(op)(x)
+    for op in (ops.newton_schulz, lambda t: ops.newton_schulz([t, t])[1]):
+        with pytest.raises(_lib.PgnnError, match="jit.trace"):
+            torch.jit.trace(op, (x,), check_trace=False)
+    assert not lib.calls
+    ops.newton_schulz([x, x])
+    assert lib.calls == ["pgnn_newton_schulz"]
