@@ -70,10 +70,10 @@ def test_recorders_of_torch_calls_are_refused(lib):
     """they would keep the result's memory and not the launch that fills it"""
     from torch.fx.experimental.proxy_tensor import make_fx
     ln, x = _frozen_layer_norm(8), torch.randn(3, 8)
-    for op in (lambda t: ops.layer_norm(t, ln), ops.newton_schulz, lambda t: ops.newton_schulz([t, t])[1]):
+    for op in (lambda t: ops.layer_norm(t, ln), lambda t: ops.newton_schulz(t), lambda t: ops.newton_schulz([t, t])[1]):
         with pytest.raises(_lib.PgnnError, match="make_fx"):
             make_fx(op)(x)
-    for op in (ops.newton_schulz, lambda t: ops.newton_schulz([t, t])[1]):
+    for op in (lambda t: ops.newton_schulz(t), lambda t: ops.newton_schulz([t, t])[1]):
         with pytest.raises(_lib.PgnnError, match="jit.trace"):
             torch.jit.trace(op, (x,), check_trace=False)
     assert not lib.calls
