@@ -1972,7 +1972,7 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     every singular value towards 1 and leave the singular vectors alone (csrc/newton_schulz.hip).  ``g``: a tensor [..., rows, cols] of
     fp32, bf16 or fp16, or a list of such matrices of any sizes (one type and device): all of them share the launches.  Returns new
     contiguous tensors of the same type, computed with the error of fp32 products whatever the type and rounded once; the same call gives
-    the same bits.  No gradient flows through it (it makes updates, not activations)."""
+    the same bits.  No gradient flows through it (it makes updates, not activations); a forward-mode tangent is refused."""
     import ctypes
     several = isinstance(g, (list, tuple))
     tensors = list(g) if several else [g]
@@ -1983,6 +1983,8 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     _refuse_proxy_trace("newton_schulz")
     if torch._C._get_tracing_state() is not None:  # (as with make_fx: no autograd function stands for the call in the graph)
         raise _lib.PgnnError("newton_schulz: torch.jit.trace cannot record it")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("newton_schulz: no rule for a forward-mode tangent (detach the matrices)")
     coef = _newton_schulz_coefficients(coefficients, steps)
     src, lds, rows, cols, dst, outs, held = [], [], [], [], [], [], []
     for t in tensors:

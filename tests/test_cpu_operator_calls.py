@@ -79,3 +79,16 @@ def test_recorders_of_torch_calls_are_refused(lib):
     assert not lib.calls
     ops.newton_schulz([x, x])
     assert lib.calls == ["pgnn_newton_schulz"]
+
+
+def test_newton_schulz_drops_no_forward_tangent(lib):
+    x = torch.randn(3, 8)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for bad in (dual, [x, dual], dual * 2):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                ops.newton_schulz(bad)
+        assert not lib.calls
+        ops.newton_schulz([x, x])
+    ops.newton_schulz(x)
+    assert lib.calls == ["pgnn_newton_schulz"] * 2
