@@ -6,6 +6,7 @@ nothing else.  Inputs must live on the GPU: there is deliberately no CPU / eager
 """
 import os
 import weakref
+from threading import get_ident
 
 import torch
 from torch.autograd import Function, forward_ad
@@ -35,9 +36,10 @@ _ws_pool = {}
 def _workspace(nbytes, device):
     """scratch for ONE C call.  Every library call finishes with its workspace before it returns
     control to the stream's next kernel (all work is enqueued in order on the current stream), so a
-    single grow-only buffer per (device, stream) replaces one allocator round trip per op."""
+    single grow-only buffer per (device, stream, host thread) replaces one allocator round trip per op.  (Per thread: ctypes lets
+    go of the interpreter's lock inside a call, so the launches of two threads' calls may alternate on one stream.)"""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    key = (idx, stream_ptr(idx))
+    key = (idx, stream_ptr(idx), get_ident())
     buf = _ws_pool.get(key)
     need = max(int(nbytes), 256)
     if buf is None or buf.numel() < need:

@@ -1,5 +1,6 @@
 """CPU: the host side of the operators' calls, the launches replaced by counters (no GPU here: nothing is launched)."""
 import contextlib
+import threading
 
 import pytest
 import torch
@@ -92,3 +93,22 @@ def test_newton_schulz_drops_no_forward_tangent(lib):
         ops.newton_schulz([x, x])
     ops.newton_schulz(x)
     assert lib.calls == ["pgnn_newton_schulz"] * 2
+
+
+def test_every_host_thread_has_a_workspace_of_its_own(lib):
+    """the launches of two threads' calls may alternate on one stream"""
+    cpu = torch.device("cpu", 0)
+    mine, others, both = ops._workspace(1000, cpu), [], threading.Barrier(2)
+
+    def other():
+        a = ops._workspace(1000, cpu)
+        both.wait()  # (two threads that live at the same time)
+        others.append((a, ops._workspace(1000, cpu)))
+
+    threads = [threading.Thread(target=other) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len({mine.data_ptr(), others[0][0].data_ptr(), others[1][0].data_ptr()}) == 3
+    assert all(a.data_ptr() == b.data_ptr() for a, b in others) and ops._workspace(1000, cpu).data_ptr() == mine.data_ptr()

@@ -1,4 +1,6 @@
 """GPU: calls of the operators that go through torch's other machinery (traces, threads, other streams)."""
+import threading
+
 import pytest
 import torch
 
@@ -23,3 +25,46 @@ def test_a_trace_of_layer_norm_gives_the_values(shape):
         junk = torch.full_like(x, float("nan"))  # what a result that nobody writes would be made of
         del junk
         assert torch.equal(traced(x), ops.layer_norm(x, ln, True) * 2)
+
+
+def test_two_host_threads_on_one_stream():
+    """calls of several launches each, from threads that share a stream: neither meets the other's planes or partial sums"""
+    from pretrain_gnns_amd import optim
+    ops = _ops()
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    work = []
+    for k in range(2):
+        mats = [torch.randn(s, generator=gen, device=DEV) for s in ((300 + 60 * k, 600), (119, 300), (700, 650))]
+        ln = torch.nn.LayerNorm(300 + 8 * k, device=DEV)
+        x = torch.randn(5000, 300 + 8 * k, generator=gen, device=DEV)
+        work.append((mats, ln, x))
+
+    def job(k):
+        mats, ln, x = work[k]
+        out = list(ops.newton_schulz(mats))
+        params = [torch.nn.Parameter(m.clone()) for m in mats]
+        for p, m in zip(params, mats):
+            p.grad = m
+        optim.Muon(params, lr=0.02).step()
+        xl = x.detach().requires_grad_(True)
+        y = ops.layer_norm(xl, ln, True)
+        return out + [p.detach() for p in params] + [y.detach()] + list(torch.autograd.grad(y, (xl, ln.weight, ln.bias), x))
+
+    want = [job(0), job(1)]
+    torch.cuda.synchronize()
+    results, start = {}, threading.Barrier(2)
+
+    def worker(k):
+        start.wait()
+        results[k] = [job(k) for _ in range(10)]
+
+    threads = [threading.Thread(target=worker, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert len(results[k]) == 10
+        for got in results[k]:
+            assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
