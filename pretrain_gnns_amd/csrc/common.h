@@ -49,8 +49,11 @@ inline int check_launch(const char* what) {
   } while (0)
 
 // dynamic LDS above the 64 KiB default needs an explicit opt-in (gfx950 has 160 KiB per CU).  The attribute
-// is sticky per function and device, so it is raised once to the largest size seen, not on every launch
-// (hipFuncSetAttribute takes the runtime's locks: microseconds that a launch-bound step does not have).
+// is sticky per function and device and belongs to the process, so it is only ever raised (raise_lds_limit: under a lock; a thread that
+// knew of its own requests alone would lower what another has asked for, and that one's next launch would be refused).  What a
+// thread has seen granted it does not ask for again (hipFuncSetAttribute takes the runtime's locks: microseconds that a
+// launch-bound step does not have).
+size_t raise_lds_limit(const void* func, int dev, size_t bytes);  // what is granted now, at least `bytes`
 inline void allow_big_lds(const void* func, size_t bytes) {
   if (bytes <= 64 * 1024) return;
   struct Seen { const void* f; int dev; size_t bytes; };
@@ -61,19 +64,11 @@ inline void allow_big_lds(const void* func, size_t bytes) {
   (void)hipGetDevice(&dev);
   for (int i = 0; i < nseen; ++i)
     if (seen[i].f == func && seen[i].dev == dev) {
-      if (seen[i].bytes >= bytes) return;
-      seen[i].bytes = bytes;
-      (void)hipFuncSetAttribute(func, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+      if (seen[i].bytes < bytes) seen[i].bytes = raise_lds_limit(func, dev, bytes);
       return;
     }
-  (void)hipFuncSetAttribute(func, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (nseen < kSlots) {
-    seen[nseen++] = Seen{func, dev, bytes};
-  } else {
-    static thread_local bool warned = false;  // still correct (the attribute is set on every launch), just slower
-    if (!warned) fprintf(stderr, "pgnn: allow_big_lds cache full (%d kernels): hipFuncSetAttribute now runs per launch\n", kSlots);
-    warned = true;
-  }
+  const size_t now = raise_lds_limit(func, dev, bytes);
+  if (nseen < kSlots) seen[nseen++] = Seen{func, dev, now};  // (else the lock is taken on every launch)
 }
 
 // A/B knobs come from the environment.  A process without any `PGNN_*` variable -- production -- takes every default at the

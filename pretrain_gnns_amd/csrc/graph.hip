@@ -9,6 +9,8 @@
 
 #include <string.h>
 
+#include <mutex>
+
 #include "common.h"
 
 extern char** environ;
@@ -31,6 +33,23 @@ static bool scan_env_for_knobs() {
   return false;
 }
 bool g_env_any = scan_env_for_knobs();
+
+size_t raise_lds_limit(const void* func, int dev, size_t bytes) {
+  struct Granted { const void* f; int dev; size_t bytes; };
+  constexpr int kSlots = 1024;
+  static std::mutex lock;
+  static Granted granted[kSlots];
+  static int count = 0;
+  std::lock_guard<std::mutex> hold(lock);
+  Granted* g = nullptr;
+  for (int i = 0; i < count && !g; ++i)
+    if (granted[i].f == func && granted[i].dev == dev) g = &granted[i];
+  if (!g && count < kSlots) *(g = &granted[count++]) = Granted{func, dev, 0};
+  if (g && g->bytes >= bytes) return g->bytes;
+  (void)hipFuncSetAttribute(func, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (g) g->bytes = bytes;
+  return bytes;
+}
 
 DeviceInfo device_info() {
   constexpr int kMaxDev = 64;

@@ -68,3 +68,20 @@ def test_two_host_threads_on_one_stream():
         assert len(results[k]) == 10
         for got in results[k]:
             assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
+
+
+def test_a_second_threads_smaller_launch_takes_no_lds_away():
+    """the same kernel with 144 KB of LDS, from another thread with 104 KB, and with 144 KB again"""
+    ops = _ops()
+    large, small = torch.randn(64, 384, device=DEV), torch.randn(64, 200, device=DEV)
+    want = ops.newton_schulz(large), ops.newton_schulz(small)
+    got = []
+
+    def other():
+        got.append(ops.newton_schulz(small))
+        torch.cuda.synchronize()
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    thread.join()
+    assert torch.equal(got[0], want[1]) and torch.equal(ops.newton_schulz(large), want[0])
