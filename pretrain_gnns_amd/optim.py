@@ -179,7 +179,8 @@ class Muon:
         optimizer_list = [Muon(weights, lr=0.02), Adam(others, lr=args.lr)]
 
     ``state[p]["momentum_buffer"]`` is p's M (zero before the first step).  A parameter without a gradient is skipped, momentum and
-    all.  lr, momentum, nesterov and weight_decay are read from ``param_groups[0]`` at every step; a captured step keeps the captured ones.
+    all.  lr, momentum, nesterov and weight_decay are read from ``param_groups[0]`` at every step; a captured step keeps the captured ones.  ns_steps, ns_coefficients, eps and
+    adjust_lr_fn are fixed when it is made.
     """
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7,
@@ -199,7 +200,7 @@ class Muon:
                 raise _lib.PgnnError("pretrain_gnns_amd.optim.Muon: contiguous fp32 parameters on one GPU only")
         if len({id(p) for p in self._own}) != len(self._own):
             raise ValueError("Muon: a parameter appears twice")
-        self.ns_steps, self.eps, self.adjust_lr_fn = int(ns_steps), float(eps), adjust_lr_fn
+        self._steps, self._eps, self._adjust = int(ns_steps), float(eps), adjust_lr_fn
         offs, total = [], 0
         for p in self._own:
             offs.append(total)
@@ -209,12 +210,17 @@ class Muon:
         self.param_groups = [{"params": self._own, "lr": lr, "weight_decay": weight_decay, "momentum": momentum, "nesterov": nesterov}]
         self._sizes, self._tables = None, None  # of the live parameters: their sizes, and what follows from sizes alone
 
+    # what the coefficients and the kept scales were made for: fixed
+    ns_steps = property(lambda self: self._steps)
+    eps = property(lambda self: self._eps)
+    adjust_lr_fn = property(lambda self: self._adjust)
+
     def zero_grad(self, set_to_none=True):
         _zero_grads(self._own, set_to_none)
 
     def _scale(self, p):
         rows, cols = p.shape
-        if self.adjust_lr_fn == "match_rms_adamw":
+        if self._adjust == "match_rms_adamw":
             return 0.2 * math.sqrt(max(rows, cols))
         return math.sqrt(max(1.0, rows / cols))
 
@@ -241,5 +247,5 @@ class Muon:
         with _on_device(dev):
             ws = _call_workspace(need, dev)
             check(lib.pgnn_muon_step(P, G, M, (ctypes.c_float * n)(*[lr * s for s in scales]), rows, cols, n, float(group["momentum"]),
-                                     int(bool(group["nesterov"])), 1.0 - lr * float(group["weight_decay"]), self._coef, self.ns_steps, self.eps,
+                                     int(bool(group["nesterov"])), 1.0 - lr * float(group["weight_decay"]), self._coef, self._steps, self._eps,
                                      ws.data_ptr(), ws.numel(), stream_ptr()), "pgnn_muon_step")

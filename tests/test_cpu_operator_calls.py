@@ -112,3 +112,14 @@ def test_every_host_thread_has_a_workspace_of_its_own(lib):
         t.join()
     assert len({mine.data_ptr(), others[0][0].data_ptr(), others[1][0].data_ptr()}) == 3
     assert all(a.data_ptr() == b.data_ptr() for a, b in others) and ops._workspace(1000, cpu).data_ptr() == mine.data_ptr()
+
+
+def test_muon_keeps_what_its_coefficients_were_made_for():
+    """ns_steps beside coefficients for another number of steps would be read past their end"""
+    from pretrain_gnns_amd import optim
+    opt = object.__new__(optim.Muon)
+    opt._steps, opt._eps, opt._adjust = 5, 1e-7, None
+    assert (opt.ns_steps, opt.eps, opt.adjust_lr_fn) == (5, 1e-7, None)
+    for name, value in (("ns_steps", 8), ("eps", 1.0), ("adjust_lr_fn", "match_rms_adamw")):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, value)
