@@ -85,3 +85,31 @@ def test_a_second_threads_smaller_launch_takes_no_lds_away():
     thread.start()
     thread.join()
     assert torch.equal(got[0], want[1]) and torch.equal(ops.newton_schulz(large), want[0])
+
+
+def test_muon_beside_torchs():
+    """the same step from gradients far above eps (that class multiplies in bf16), and half of it where |U| is eps: eps is added"""
+    from pretrain_gnns_amd import optim
+    gen = torch.Generator().manual_seed(0)
+    w, g = torch.randn(48, 96, generator=gen), torch.randn(48, 96, generator=gen)
+    ours, theirs = torch.nn.Parameter(w.clone().to(DEV)), torch.nn.Parameter(w.clone())
+    a = optim.Muon([ours], lr=1.0, weight_decay=0.1, momentum=0.9)
+    b = torch.optim.Muon([theirs], lr=1.0, weight_decay=0.1, momentum=0.9)
+    for k in range(3):
+        ours.grad, theirs.grad = (g * (1 + k)).to(DEV), g * (1 + k)
+        a.step()
+        b.step()
+        # M is their average times 1 / (1 - momentum): three roundings of either
+        m, n = a.state[ours]["momentum_buffer"].cpu() * 0.1, b.state[theirs]["momentum_buffer"]
+        assert ((m - n).abs() <= 8 * 2.0 ** -24 * (k + 1) * n.abs().max()).all()
+        # five steps of three products in bf16, each term off by 2^-8 at most (as a random walk far less than 15 * 2^-8 of the direction)
+        step = (theirs.detach() - w).norm()
+        assert (ours.detach().cpu() - theirs.detach()).norm() <= 15 * 2.0 ** -8 * step
+    # one linear step of which X_0 = U / (|U| + eps) is the result
+    u = g * 1.9  # G + 0.9 M, M = G
+    for eps, share in ((1e-7, 1.0), (u.norm().item(), 0.5), (3 * u.norm().item(), 0.25)):
+        p = torch.nn.Parameter(torch.zeros(48, 96, device=DEV))
+        p.grad = g.to(DEV)
+        optim.Muon([p], lr=1.0, weight_decay=0.0, momentum=0.9, ns_coefficients=(1.0, 0.0, 0.0), ns_steps=1, eps=eps).step()
+        want = -(u.double() / u.double().norm()) * share
+        assert (p.detach().cpu().double() - want).norm() <= 2.0 ** -19 * share  # planes of 22 bits, eps and the norm rounded to fp32
