@@ -113,3 +113,18 @@ def test_muon_beside_torchs():
         optim.Muon([p], lr=1.0, weight_decay=0.0, momentum=0.9, ns_coefficients=(1.0, 0.0, 0.0), ns_steps=1, eps=eps).step()
         want = -(u.double() / u.double().norm()) * share
         assert (p.detach().cpu().double() - want).norm() <= 2.0 ** -19 * share  # planes of 22 bits, eps and the norm rounded to fp32
+
+
+def test_a_graph_from_before_a_muon_step_is_refused():
+    """the step writes to the parameters: a backward pass that still wants their old values has to notice, as after any in-place update"""
+    from pretrain_gnns_amd import optim
+    p = torch.nn.Parameter(torch.randn(8, 12, device=DEV))
+    opt = optim.Muon([p], lr=0.02)
+    p.grad = torch.randn(8, 12, device=DEV)
+    x = torch.randn(5, 8, device=DEV, requires_grad=True)
+    loss = (x @ p).sum()
+    before = p._version
+    opt.step()
+    assert p._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
