@@ -243,7 +243,10 @@ class Muon:
             self._tables = rows, cols, lib.pgnn_newton_schulz_workspace_bytes(rows, cols, n), [self._scale(p) for p in live]
             self._sizes = sizes
         rows, cols, need, scales = self._tables
-        P, G, M = ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (live, grads, momenta))
+        written = [t.data_ptr() for t in live + momenta]
+        if len(set(written)) != 2 * n:  # (all matrices of a call are updated at the same time)
+            raise _lib.PgnnError("pretrain_gnns_amd.optim.Muon: two parameters, or momentum buffers, at one place in memory")
+        P, M, G = (ctypes.c_void_p * n)(*written[:n]), (ctypes.c_void_p * n)(*written[n:]), (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
         group = self.param_groups[0]
         lr = float(group["lr"])
         with _on_device(dev):

@@ -128,3 +128,23 @@ def test_a_graph_from_before_a_muon_step_is_refused():
     assert p._version > before
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_muon_refuses_two_parameters_in_one_memory():
+    from pretrain_gnns_amd import _lib, optim
+    w = torch.randn(8, 12, device=DEV)
+    a, b = torch.nn.Parameter(w), torch.nn.Parameter(w)
+    c, d = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.clone())
+    for pair, tie in (((a, b), False), ((c, d), True)):
+        opt = optim.Muon(pair, lr=0.02)
+        for p in pair:
+            p.grad = torch.ones(8, 12, device=DEV)
+        if tie:
+            opt.state[c]["momentum_buffer"] = opt.state[d]["momentum_buffer"]
+        with pytest.raises(_lib.PgnnError, match="one place"):
+            opt.step()
+    assert torch.equal(a, w) and torch.equal(c, w) and torch.equal(d, w)
+    b.grad = None  # one of them alone
+    before = w.clone()
+    optim.Muon((a, b), lr=0.02).step()
+    assert torch.equal(a, b) and not torch.equal(a, before)
