@@ -791,10 +791,13 @@ class _on_device:
             torch.cuda.set_device(self.before)
 
 
+_POOLED_BYTES = 32 << 20  # (an allocation of this size costs some microseconds, beside a call of hundreds)
+
+
 def _call_workspace(nbytes, device):
     """``_workspace``, but a captured call gets a buffer of its own from the graph's memory: two graphs captured on one stream may
-    be replayed side by side, and the pool's buffer would be shared by them"""
-    if torch.cuda.is_current_stream_capturing():
+    be replayed side by side, and the pool's buffer would be shared by them.  So does a call that needs much: the pool's buffers stay"""
+    if nbytes > _POOLED_BYTES or torch.cuda.is_current_stream_capturing():
         return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
     return _workspace(nbytes, device)
 

@@ -123,3 +123,14 @@ def test_muon_keeps_what_its_coefficients_were_made_for():
     for name, value in (("ns_steps", 8), ("eps", 1.0), ("adjust_lr_fn", "match_rms_adamw")):
         with pytest.raises(AttributeError):
             setattr(opt, name, value)
+
+
+def test_a_large_workspace_goes_back(lib):
+    """what a call needs beyond the pool's size is not kept for the process"""
+    cpu = torch.device("cpu", 0)
+    small = ops._call_workspace(1 << 20, cpu)
+    assert ops._call_workspace(1 << 20, cpu).data_ptr() == small.data_ptr()
+    large = ops._call_workspace(100 << 20, cpu)
+    assert large.numel() == 100 << 20
+    assert sum(b.numel() for b in ops._ws_pool.values()) < 100 << 20
+    assert ops._call_workspace(1 << 20, cpu).data_ptr() == small.data_ptr()
