@@ -960,6 +960,8 @@ def use_layer_norm(module):
                 with torch.no_grad():
                     new.weight.copy_(child.weight)
                     new.bias.copy_(child.bias)
+                new.weight.requires_grad_(child.weight.requires_grad)
+                new.bias.requires_grad_(child.bias.requires_grad)
             setattr(module, name, new.train(child.training))
         else:
             use_layer_norm(child)

@@ -134,3 +134,11 @@ def test_a_large_workspace_goes_back(lib):
     assert large.numel() == 100 << 20
     assert sum(b.numel() for b in ops._ws_pool.values()) < 100 << 20
     assert ops._call_workspace(1 << 20, cpu).data_ptr() == small.data_ptr()
+
+
+def test_use_layer_norm_leaves_frozen_gains_frozen():
+    net = torch.nn.Sequential(torch.nn.BatchNorm1d(4), torch.nn.BatchNorm1d(4))
+    net[0].weight.requires_grad_(False)
+    net[1].bias.requires_grad_(False)
+    ops.use_layer_norm(net)
+    assert [p.requires_grad for p in net.parameters()] == [False, True, True, False]
