@@ -949,22 +949,27 @@ def norm(x, module, relu=False, drop_p=0.0):
 
 
 def use_layer_norm(module):
-    """replace every ``torch.nn.BatchNorm1d`` below ``module`` by a ``torch.nn.LayerNorm`` of its width, eps and gains: the networks
-    of chem.model and bio.model then normalise every node over its features.  The gains are new parameters (build the optimizers
-    afterwards); state-dict keys of weight and bias stay, those of the running statistics go."""
-    for name, child in list(module.named_children()):
-        if type(child) is torch.nn.BatchNorm1d:
-            where = dict(device=child.weight.device, dtype=child.weight.dtype) if child.affine else {}
-            new = torch.nn.LayerNorm(child.num_features, eps=child.eps, elementwise_affine=child.affine, **where)
-            if child.affine:
-                with torch.no_grad():
-                    new.weight.copy_(child.weight)
-                    new.bias.copy_(child.bias)
-                new.weight.requires_grad_(child.weight.requires_grad)
-                new.bias.requires_grad_(child.bias.requires_grad)
-            setattr(module, name, new.train(child.training))
-        else:
-            use_layer_norm(child)
+    """replace every ``torch.nn.BatchNorm1d`` below ``module`` (parallel.ExactBatchNorm1d among them) by a ``torch.nn.LayerNorm`` of its
+    width, eps and gains: the networks of chem.model and bio.model then normalise every node over its features.  One that is in several
+    places is replaced by one.  The gains are new parameters (build the optimizers afterwards), frozen where they were; state-dict keys
+    of weight and bias stay, those of the running statistics go."""
+    made = {}
+    for parent in list(module.modules()):
+        for name, child in parent._modules.items():
+            if not isinstance(child, torch.nn.BatchNorm1d):
+                continue
+            new = made.get(child)
+            if new is None:
+                where = dict(device=child.weight.device, dtype=child.weight.dtype) if child.affine else {}
+                new = made[child] = torch.nn.LayerNorm(child.num_features, eps=child.eps, elementwise_affine=child.affine, **where)
+                if child.affine:
+                    with torch.no_grad():
+                        new.weight.copy_(child.weight)
+                        new.bias.copy_(child.bias)
+                    new.weight.requires_grad_(child.weight.requires_grad)
+                    new.bias.requires_grad_(child.bias.requires_grad)
+                new.train(child.training)
+            parent._modules[name] = new
     return module
 
 

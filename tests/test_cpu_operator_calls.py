@@ -142,3 +142,15 @@ def test_use_layer_norm_leaves_frozen_gains_frozen():
     net[1].bias.requires_grad_(False)
     ops.use_layer_norm(net)
     assert [p.requires_grad for p in net.parameters()] == [False, True, True, False]
+
+
+def test_use_layer_norm_finds_every_batch_norm():
+    """one that is in two places (and stays one), and the data-parallel form"""
+    from pretrain_gnns_amd import parallel
+    shared = torch.nn.BatchNorm1d(4)
+    net = torch.nn.ModuleDict({"a": shared, "b": torch.nn.Sequential(torch.nn.Linear(4, 4), shared), "c": torch.nn.BatchNorm1d(4, affine=False)})
+    ops.use_layer_norm(net)
+    assert type(net["a"]) is torch.nn.LayerNorm and net["a"] is net["b"][1]
+    assert type(net["c"]) is torch.nn.LayerNorm and net["c"].weight is None
+    exact = parallel.use_exact_batchnorm(torch.nn.Sequential(torch.nn.BatchNorm1d(4)))
+    assert type(ops.use_layer_norm(exact)[0]) is torch.nn.LayerNorm
