@@ -821,7 +821,7 @@ def _last_axis_rows(t, dim):
 
 def _layer_norm_fwd(x, gamma, beta, dim, eps, relu, keep):
     rows2d = _last_axis_rows(x, dim)
-    rows = rows2d.size(0)
+    rows = int(rows2d.size(0))  # (under torch.jit.trace a size is a tensor)
     y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)  # (empty_like: half of empty's host time)
     stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
     mean = stats.data_ptr() if keep and rows else None

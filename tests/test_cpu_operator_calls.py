@@ -10,13 +10,17 @@ from pretrain_gnns_amd import _lib, ops
 
 
 class _Counting:
-    """the library as far as these tests go: workspaces of 1 KB, calls that do nothing, counted by name"""
+    """the library as far as these tests go: workspaces of 1 KB, calls that convert their arguments and do nothing, counted by name"""
 
     def __init__(self):
         self.calls = []
 
     def __getattr__(self, name):
         def call(*args):
+            kinds = _lib.PROTOTYPES[name][1]
+            assert len(args) == len(kinds)
+            for kind, value in zip(kinds, args):
+                kind.from_param(value)
             if name.endswith("workspace_bytes"):
                 return 1024
             self.calls.append(name)
