@@ -211,9 +211,9 @@ __device__ __forceinline__ float4 f4_add(float4 a, float4 b) {
 __device__ __forceinline__ float4 f4_scale(float4 a, float s) {
   return make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
 }
-// a . b with every product rounded before it is added, and p a + q b likewise: what the compiler made of these sums while it paired
-// the products in packed multiplications.  Those are off (build.py); without this it would fuse one product of each sum into the
-// addition, and results that were pinned before would move in the last bit.
+// Sums of products whose rounding is pinned.  The compiler used to choose what it fused by how it paired products in packed instructions;
+// those are off (build.py), and left to itself it would now choose otherwise and move results in the last bit.
+// a . b with every product rounded before it is added, and p a + q b likewise:
 __device__ __forceinline__ float f4_dot(float4 a, float4 b) {
 #pragma clang fp contract(off)
   return (a.x * b.x + a.y * b.y) + (a.z * b.z + a.w * b.w);
@@ -222,6 +222,8 @@ __device__ __forceinline__ float mix(float p, float a, float q, float b) {
 #pragma clang fp contract(off)
   return p * a + q * b;
 }
+// a b, not rounded, on top of c d, rounded
+__device__ __forceinline__ float fma_pair(float a, float b, float c, float d) { return fmaf(a, b, c * d); }
 __device__ __forceinline__ float4 f4_zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
 
 // Results one block publishes and ANOTHER block of the same launch reads: agent-scope accesses -- write-through stores, loads that

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kCtxThreads) k_ctx_scores(const float* __restr
   for (int k = 0; k <= neg; ++k) {
     const int j = k == 0 ? g : (g + k) % B;
     const float4 c = on ? *reinterpret_cast<const float4*>(ctx + (int64_t)j * dim + 4 * t) : f4_zero();
-    red[k][t] = f4_dot(s, c);
+    red[k][t] = fma_pair(s.y, c.y, s.x, c.x) + fma_pair(s.w, c.w, s.z, c.z);
   }
   __syncthreads();
   for (int h = kCtxThreads / 2; h > 0; h >>= 1) {  // fixed tree: the same order every run
