@@ -35,7 +35,6 @@ __device__ __forceinline__ float wave_sum(float v) {
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
   return v;
 }
-__device__ __forceinline__ float dot4(float4 a, float4 b) { return (a.x * b.x + a.y * b.y) + (a.z * b.z + a.w * b.w); }
 
 inline int grid_rows(int64_t rows, int per_block) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, per_block), (int64_t)num_cu() * 16));
@@ -51,8 +50,10 @@ __global__ void __launch_bounds__(kBlock) k_rowdot(const float* __restrict__ xh,
       float ai = 0.f, aj = 0.f;
       for (int c = lane; c < d4; c += 64) {
         const float4 v = reinterpret_cast<const float4*>(xh + i * ldx + h * d)[c];
-        ai += dot4(v, reinterpret_cast<const float4*>(att + h * 2 * d)[c]);
-        aj += dot4(v, reinterpret_cast<const float4*>(att + h * 2 * d + d)[c]);
+        const float4 a = reinterpret_cast<const float4*>(att + h * 2 * d)[c], b = reinterpret_cast<const float4*>(att + h * 2 * d + d)[c];
+        // (which product of a pair is rounded is part of the result: fma_pair)
+        ai += fma_pair(v.x, a.x, v.y, a.y) + fma_pair(v.z, a.z, v.w, a.w);
+        aj += fma_pair(v.y, b.y, v.x, b.x) + fma_pair(v.w, b.w, v.z, b.z);
       }
       ai = wave_sum(ai);
       aj = wave_sum(aj);
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(kBlock) k_gat_edge_dot(const float* __restrict
               m.x = fmaf(f[k], tv.x, m.x); m.y = fmaf(f[k], tv.y, m.y); m.z = fmaf(f[k], tv.z, m.z); m.w = fmaf(f[k], tv.w, m.w);
             }
           }
-          acc[h] += dot4(gv, m);
+          // (as in k_rowdot)
+          acc[h] += fma_pair(gv.y, m.y, gv.x, m.x) + fma_pair(gv.z, m.z, gv.w, m.w);
         }
       }
 #pragma unroll

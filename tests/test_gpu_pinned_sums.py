@@ -49,6 +49,41 @@ def test_the_oracle_tells_the_orders_apart():
     assert all(a != b for k, a in enumerate(forms) for b in forms[:k])
 
 
+def test_gat_logits_and_their_gradients():
+    from pretrain_gnns_amd import _lib, ops
+    n, d, heads = 30, 4, 2
+    gen = torch.Generator().manual_seed(0)
+    edge_index = torch.randint(0, n, (2, 50), generator=gen).to(DEV)
+    edge_attr = torch.stack([torch.randint(0, 4, (50,), generator=gen), torch.randint(0, 3, (50,), generator=gen)], 1).to(DEV)
+    g = ops.build_chem_graph(edge_index, edge_attr, n)
+    xh, att, gout = _normal(n, heads * d, seed=1), _normal(heads, 2 * d, seed=2), _normal(n, d, seed=3)
+    zero = torch.zeros(6, heads * d, device=DEV), torch.zeros(3, heads * d, device=DEV)  # (the bond tables: m = xh + 0)
+    dx, da, dg = xh.to(DEV), att.to(DEV), gout.to(DEV)
+    ctab, bias = torch.zeros(18, heads, device=DEV), torch.zeros(d, device=DEV)
+    new = lambda *s: torch.zeros(*s, device=DEV)
+    scores, z, alpha, cfa, out = new(n, 2 * heads), new(g.e + n, heads), new(g.e + n, heads), new(heads, n, 9), new(n, d)
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()
+    graph = (p(g.in_ptr), p(g.in_src), p(g.in_code))
+    assert lib.pgnn_gat_fwd(p(dx), heads * d, *graph, p(zero[0]), p(zero[1]), p(ctab), None, None, None, 0, p(da), p(bias), 0.2, p(scores), p(z),
+                            p(alpha), p(cfa), p(out), d, n, d, st) == 0
+    x, a = xh.view(n, heads, d).numpy(), att.numpy()
+    want = [[_first_fused(x[i, h], a[h, :d]) for h in range(heads)] + [_second_fused(x[i, h], a[h, d:]) for h in range(heads)] for i in range(n)]
+    assert np.array_equal(scores.cpu().numpy(), np.array(want, dtype=np.float32))
+
+    # an edge's weight gradient dalpha = g . m / 2.  The call hands out dz = alpha (dalpha - sum alpha dalpha): with every alpha 2^-60 the
+    # second term is far below half a step of the first, and with z > 0 nothing else touches it
+    z.fill_(1.0)
+    alpha.fill_(2.0 ** -60)
+    dz, dsd, czf, wout, dxh = new(g.e + n, heads), new(heads, n, 2), new(heads, n, 9), new(max(g.e, 1), heads), new(n, heads * d)
+    assert lib.pgnn_gat_bwd(p(dg), d, p(dx), heads * d, *graph, p(g.out_ptr), p(g.out_dst), p(zero[0]), p(zero[1]), None, None, None, 0, p(da), 0.2,
+                            p(z), p(alpha), p(dz), p(dsd), p(czf), p(wout), p(dxh), heads * d, n, d, st) == 0
+    ptr, src, gn = g.in_ptr.tolist(), g.in_src.tolist(), gout.numpy()
+    want = [[_ends_rounded(gn[i], x[src[q] if q < ptr[i + 1] else i, h]) / np.float32(2) for h in range(heads)]
+            for i in range(n) for q in range(ptr[i], ptr[i + 1] + 1)]
+    assert np.array_equal(dz.cpu().numpy() * np.float32(2.0 ** 60), np.array(want, dtype=np.float32))
+
+
 def test_context_prediction_scores():
     from pretrain_gnns_amd import ops
     for seed in range(6):
