@@ -33,3 +33,22 @@ def _reload_library_env_after_the_test():
     lib = getattr(mod, "_lib", None) if mod is not None else None
     if lib is not None:
         lib.pgnn_reload_env()
+
+
+# Host results of the GPU tests: how torch cuts a sum into parts, and so its last bits, depends on the number of host threads.  With 12 or 16
+# of them one fp32 BatchNorm pre-activation of those that are compared (3.8e-8 in 64 bits) falls on the other side of zero, and its ReLU's
+# gradient with it; with 4 every one of them has the sign that it has in 64 bits (test_cpu_host_reference.py)
+HOST_THREADS = 4
+
+
+@pytest.fixture(autouse=True)
+def _host_threads_of_gpu_tests(request):
+    if "gpu" not in request.keywords:
+        yield
+        return
+    import torch
+
+    before = torch.get_num_threads()
+    torch.set_num_threads(HOST_THREADS)
+    yield
+    torch.set_num_threads(before)
