@@ -26,7 +26,7 @@ using namespace pgnn;
 
 namespace {
 
-constexpr int kMaxJobs = 48;         // matrices per launch (the job table travels in the kernel arguments: 3.4 KB at most)
+constexpr int kMaxJobs = 48;         // matrices per launch (their table travels in the kernel arguments: kArguments)
 constexpr int kMaxSteps = 32;
 constexpr int kMaxParts = 1024;      // partial sums of squares per matrix (256: one wave per SIMD, 4096 x 4096 40 us)
 constexpr int64_t kNormPart = 4096;  // elements per partial sum, at least
@@ -116,6 +116,10 @@ struct Bounds {             // of the iteration on [0, 1]: max |p| after t steps
   int steps;
   float eps;
 };
+
+// k_ns_tiny takes all of these (3 964 bytes), the other kernels fewer; a launch's arguments are 4 KB at most
+constexpr size_t kArguments = sizeof(Jobs) + sizeof(Sources) + sizeof(Results) + sizeof(MuonArgs) + sizeof(Bounds);
+static_assert(kArguments <= 4096, "fewer matrices per launch");
 
 // the job of a workgroup: every lane loads one, a ballot finds the last that begins at or before this workgroup, its fields are read from
 // that lane.  One round trip to the kernel arguments; a bisection and a load of what it found are five
