@@ -470,11 +470,11 @@ void by_vectors(int nv, const Args& a) {
 
 template <typename T, typename W, typename Args>
 void by_width(const Args& a) {
-  constexpr int VE = Pack<T>::n, MAXNV = 32 / VE;
+  constexpr int VE = Pack<T>::n, FEW = 31 / VE;  // (vectors per lane: fewer than 32 values, on 256 lanes up to kRegDim columns)
   const int lpr = lanes_per_row(a.dim, VE), nv = (int)ceil_div(a.dim, lpr * VE);
-  if (lpr == 16) by_vectors<T, W, 16, MAXNV>(nv, a);
-  else if (lpr == 64) by_vectors<T, W, 64, MAXNV>(nv, a);
-  else by_vectors<T, W, 256, MAXNV>(nv, a);
+  if (lpr == 16) by_vectors<T, W, 16, FEW>(nv, a);
+  else if (lpr == 64) by_vectors<T, W, 64, FEW, Args, FEW / 4 + 1>(nv, a);  // (more than 16 or 64 lanes hold with FEW)
+  else by_vectors<T, W, 256, kRegDim / 256 / VE, Args, FEW / 4 + 1>(nv, a);
 }
 
 template <typename T, typename W>
