@@ -392,9 +392,11 @@ int pgnn_adam_step(float* const* params, const float* const* grads, const int64_
  * the reference, which knows Adam only).  For each of `count` matrices G [rows, cols] (host arrays of device pointers, sizes and leading
  * dimensions in elements; any count, sizes 0 to 32768):
  *   X = G / (|G|_F + eps), transposed while rows > cols; per step t, with (a, b, c) = coefficients[3 t .. 3 t + 2] (host, fp32):
- *   A = X X^T, X <- a X + (b A + c A A) X;  result = X, dense [rows, cols] of the same `type` (PGNN_F32 / PGNN_BF16 / PGNN_F16), rounded once
- * with the error of fp32 products throughout.  dst[j] may be src[j].  1 to 32 steps; coefficients under which the bound on X's singular
- * values (they start in [0, 1]) passes 2^20 are refused.  A matrix of zeros gives zeros (eps > 0), one with a NaN or an infinity NaN throughout;
+ *   A = X X^T, X <- a X + (b A + c A A) X;  result = X, dense [rows, cols] of the same `type` (PGNN_F32 / PGNN_BF16 / PGNN_F16), rounded once.
+ * Operands are held to 2^-23 of the value, or 2^-37 of the bound u on X's singular values (2^-37 u^2 for A) where that is more, sums are fp32: in
+ * the Frobenius and the spectral norm the error of an iteration on fp32 products.  Not row by row: a row below 2^-16 of the others' size
+ * keeps fewer than 22 bits (rows graded from 1 to 1e-6, 200 x 400: the weakest are 2.5e-4 of themselves off, with fp32 products 1e-5).
+ * dst[j] may be src[j].  1 to 32 steps; coefficients under which u (it starts at 1) passes 2^20 are refused.  A matrix of zeros gives zeros (eps > 0), one with a NaN or an infinity NaN throughout;
  * what is left of values of X that start below 2^-60 (a norm far below eps) is lost.
  * The same workspace serves both calls; matrices are taken in chunks (at most 48, and 2 GiB of workspace unless one needs more).
  * pgnn_muon_step: fp32, dense; per matrix  M <- mu M + G;  U = nesterov ? G + mu M : M;  p <- keep p - rates[j] orthogonal(U)

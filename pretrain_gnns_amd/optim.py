@@ -169,7 +169,7 @@ class Muon:
     Per matrix  M <- momentum M + G;  U = G + momentum M (nesterov) or M;  O = ops.newton_schulz(U, ns_steps, ns_coefficients, eps);
     p <- p (1 - lr weight_decay) - lr s O  with s = sqrt(max(1, rows / cols)) (``adjust_lr_fn`` None or "original") or
     0.2 sqrt(max(rows, cols)) ("match_rms_adamw": updates as large as Adam's).  The arguments are those of torch.optim.Muon, and so is the
-    step but for three things.  The products carry fp32's error where that class multiplies in bf16.  ``eps`` is added to the norm where that
+    step but for three things.  The direction carries fp32's error (in the norm: ops.newton_schulz) where that class multiplies in bf16.  ``eps`` is added to the norm where that
     class takes the larger of the two.  M is a sum where that class keeps an average (this M times 1 - momentum), which is the same direction
     U / |U| but reaches eps at gradients 1 / (1 - momentum) times smaller: both matter for norms near eps only.
 

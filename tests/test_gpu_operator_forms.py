@@ -156,6 +156,27 @@ def test_muon_small_matrices_apart_from_large_ones(shapes):
     _muon_check(shapes)
 
 
+@pytest.mark.parametrize("rows,cols", [(40, 300), (200, 400), (400, 500), (400, 200)])
+@pytest.mark.parametrize("low", [1e-3, 1e-6])
+def test_newton_schulz_of_graded_rows(rows, cols, low):
+    """row by row (column by column of a tall matrix) what the planes promise: beside what fp32 products lose, every entry of X, A and B is
+    off by up to 2^-37 of its bound, u <= 1.21, u^2 and 2.81.  Of a weak row, which grows by 3.4445 a step, a step adds 2^-37 (sqrt(n) u +
+    sqrt(k) (4.775 u^3 + 2 * 2.0315 u^5 + 2.81 u)) at most, and a step's share grows as the row does: 1 / (1 - 1 / 3.4445) = 1.41 of the first's"""
+    g = torch.randn(rows, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    k, n = min(rows, cols), max(rows, cols)
+    grade = torch.logspace(0, math.log10(low), k, device=DEV)
+    g = g * (grade[:, None] if rows <= cols else grade)
+    out, want, host = _ops().newton_schulz(g).double(), _iterate(g.double()), _iterate(g).double()
+    axis = 1 if rows <= cols else 0
+    u = 1.21
+    planes = 1.41 * 3.4445 ** 5 * 2.0 ** -37 * (math.sqrt(n) * u + math.sqrt(k) * (4.775 * u ** 3 + 2 * 2.0315 * u ** 5 + 2.81 * u))
+    off, size = (out - want).norm(dim=axis), want.norm(dim=axis)
+    assert (off <= 3 * (host - want).norm(dim=axis) + 2.0 ** -18 * size + planes).all()
+    assert (out - want).norm().item() <= 3 * (host - want).norm().item() + 2.0 ** -18 * want.norm().item()  # and in the norm without that
+    if low == 1e-3:
+        assert (off / size).max().item() <= 2.0 ** -14  # (2^-10 of the largest: still within the planes' 22 bits)
+
+
 # ------------------------------------------------------------------------------------------------------------ layer norm
 def _layer_norm_check(rows, dim, dtype, gains, relu, seed=0):
     """per element, as the roundings of the arithmetic bound it.  A row's mean: at most 32 values in a lane and 12 partial sums, off by
