@@ -254,4 +254,5 @@ class Muon:
             check(lib.pgnn_muon_step(P, G, M, (ctypes.c_float * n)(*[lr * s for s in scales]), rows, cols, n, float(group["momentum"]),
                                      int(bool(group["nesterov"])), 1.0 - lr * float(group["weight_decay"]), self._coef, self._steps, self._eps,
                                      ws.data_ptr(), ws.numel(), stream_ptr()), "pgnn_muon_step")
-        torch.autograd.graph.increment_version(live + momenta)  # (a graph that still holds them must notice)
+        # (a graph that still holds them must notice; tensors made in inference mode are in no graph and have no counter)
+        torch.autograd.graph.increment_version([t for t in live + momenta if not t.is_inference()])

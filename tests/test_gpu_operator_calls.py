@@ -148,3 +148,22 @@ def test_muon_refuses_two_parameters_in_one_memory():
     before = w.clone()
     optim.Muon((a, b), lr=0.02).step()
     assert torch.equal(a, b) and not torch.equal(a, before)
+
+
+def test_muon_made_and_stepped_in_inference_mode():
+    """tensors without version counters"""
+    from pretrain_gnns_amd import optim
+    w, g = torch.randn(8, 12, device=DEV), torch.randn(8, 12, device=DEV)
+    outside, kept = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.clone())
+    with torch.inference_mode():
+        inside = torch.nn.Parameter(w.clone())
+        opts = [optim.Muon([inside], lr=0.02), optim.Muon([outside], lr=0.02)]
+        inside.grad = g.clone()
+    outside.grad = kept.grad = g
+    plain = optim.Muon([kept], lr=0.02)
+    for _ in range(2):
+        plain.step()
+        opts[1].step()
+        with torch.inference_mode():
+            opts[0].step()
+    assert torch.equal(outside, kept) and torch.equal(inside, kept)
