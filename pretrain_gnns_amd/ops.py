@@ -802,13 +802,13 @@ def _call_workspace(nbytes, device):
     return _workspace(nbytes, device)
 
 
-_PROXY_MODE = torch._C._TorchDispatchModeKey.PROXY
+_dispatch_mode, _tracing_state, _PROXY_MODE = torch._C._get_dispatch_mode, torch._C._get_tracing_state, torch._C._TorchDispatchModeKey.PROXY
 
 
 def _refuse_proxy_trace(what):
-    """make_fx records torch's own calls only: the result's memory would be in its graph, the kernel that fills it would not"""
-    if torch._C._get_dispatch_mode(_PROXY_MODE) is not None:
-        raise _lib.PgnnError("%s: make_fx cannot record it" % what)
+    """make_fx (``_dispatch_mode(_PROXY_MODE)`` is set) records torch's own calls only: the result's memory would be in its graph, the
+    kernel that fills it would not"""
+    raise _lib.PgnnError("%s: make_fx cannot record it" % what)
 
 
 def _last_axis_rows(t, dim):
@@ -901,7 +901,8 @@ def layer_norm(x, ln, relu=False):
     node to the stream of the result that still holds it)."""
     gamma, beta = ln.weight, ln.bias
     require_cuda(x, gamma, beta)
-    _refuse_proxy_trace("layer_norm")
+    if _dispatch_mode(_PROXY_MODE) is not None:
+        _refuse_proxy_trace("layer_norm")
     shape = ln.normalized_shape
     if len(shape) == 1:
         dim = shape[0]
@@ -929,7 +930,7 @@ def layer_norm(x, ln, relu=False):
             raise _lib.PgnnError("layer_norm: contiguous gains only")
     relu = 1 if relu else 0
     # the tape has to see the call where gradients are recorded, and where a forward-mode tangent (which it refuses) or a trace passes through
-    grad = forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None or (
+    grad = forward_ad._current_level >= 0 or _tracing_state() is not None or (
         torch.is_grad_enabled() and (x.requires_grad or (gamma is not None and gamma.requires_grad) or (beta is not None and beta.requires_grad)))
     if x.device.index != torch.cuda.current_device():
         with torch.cuda.device(x.device):
@@ -1993,8 +1994,9 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
         return []
     first = tensors[0]
     require_cuda(*tensors)
-    _refuse_proxy_trace("newton_schulz")
-    if torch._C._get_tracing_state() is not None:  # (as with make_fx: no autograd function stands for the call in the graph)
+    if _dispatch_mode(_PROXY_MODE) is not None:
+        _refuse_proxy_trace("newton_schulz")
+    if _tracing_state() is not None:  # (as with make_fx: no autograd function stands for the call in the graph)
         raise _lib.PgnnError("newton_schulz: torch.jit.trace cannot record it")
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("newton_schulz: no rule for a forward-mode tangent (detach the matrices)")
