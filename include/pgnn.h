@@ -396,8 +396,9 @@ int pgnn_adam_step(float* const* params, const float* const* grads, const int64_
  * Operands are held to 2^-23 of the value, or 2^-37 of the bound u on X's singular values (2^-37 u^2 for A) where that is more, sums are fp32: in
  * the Frobenius and the spectral norm the error of an iteration on fp32 products.  Not row by row: a row below 2^-16 of the others' size
  * keeps fewer than 22 bits (rows graded from 1 to 1e-6, 200 x 400: the weakest are 2.5e-4 of themselves off, with fp32 products 1e-5).
- * dst[j] may be src[j].  1 to 32 steps; coefficients under which u (it starts at 1) passes 2^20 are refused.  A matrix of zeros gives zeros (eps > 0), one with a NaN or an infinity NaN throughout;
- * what is left of values of X that start below 2^-60 (a norm far below eps) is lost.
+ * dst[j] may be src[j]; what a call writes must not overlap otherwise (all matrices are worked on at the same time).  1 to 32 steps;
+ * coefficients under which u (it starts at 1) passes 2^20 are refused.  A matrix of zeros gives zeros (eps > 0), one with a NaN or an
+ * infinity NaN throughout; what is left of values of X that start below 2^-60 (a norm far below eps) is lost.
  * The same workspace serves both calls; matrices are taken in chunks (at most 48, and 2 GiB of workspace unless one needs more).
  * pgnn_muon_step: fp32, dense; per matrix  M <- mu M + G;  U = nesterov ? G + mu M : M;  p <- keep p - rates[j] orthogonal(U)
  * (keep = 1 - lr weight_decay; rates: host).  No allocation; the same call gives the same bits (how a long sum is cut depends on all

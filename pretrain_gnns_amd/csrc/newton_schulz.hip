@@ -471,8 +471,8 @@ __device__ __forceinline__ void read_turned8(uint32_t p, uint32_t q, f16x8 (&ph)
 // TT/2; two fetch P and two fetch Q by LDS DMA, STAGES - 1 of the group's stages ahead.  A stage is 32 deep: of A A and B X, where l runs
 // along the operands' rows, a column of TT/16 blocks of each; of X X^T, where l runs down the rows of X^T, two rows of TT/32 blocks, whose
 // fragments (8 l of one column per lane) are two ds_read_b64_tr_b16 each: a 16-lane group hands over 4 rows x 16 columns turned.
-// Bound by the matrix pipes and what keeps them waiting at the barriers (busy 0.65-0.72 of the time): 4096 x 4096 A 190 us, 1 120 TFLOP/s on
-// planes; A A 196; B X 319, 1 290; the library's fp16 product of 8192 1 363 beside it.
+// Bound by the matrix pipes and what keeps them waiting at the barriers (busy 0.65-0.72 of the time): 4096 x 4096 A 194 us, 1 100 TFLOP/s on
+// planes (diagonal tiles whole); A A 200, 1 060; B X 329, 1 250, the last one 344, 1 200; the library's fp16 product of 8192 1 330 beside it.
 template <int TT, int STAGES, int G, int PHASE, typename TO, bool MUON>
 __global__ void __launch_bounds__(256 * G) k_ns_product(Jobs jobs, Last<PHASE> to, Muon<MUON> mu, int step, float ca, float cb, float cc) {
   constexpr int MI = TT / 32, OPER = TT * kBK * 4, STAGE = 2 * OPER, NJ = TT / 16;
