@@ -167,3 +167,40 @@ def test_muon_made_and_stepped_in_inference_mode():
         with torch.inference_mode():
             opts[0].step()
     assert torch.equal(outside, kept) and torch.equal(inside, kept)
+
+
+@pytest.mark.parametrize("shapes", [[(3, 300), (64, 384), (33, 1)], [(119, 301), (300, 600), (321, 35)], [(700, 651), (333, 1030)]])
+def test_muon_with_weights_anywhere_in_memory(shapes):
+    """parameters, gradients and momenta as parts of a buffer at any multiple of four bytes: the same bits as with tensors of their own, and
+    what lies between them stays as it was"""
+    from pretrain_gnns_amd import optim
+    gen = torch.Generator(device=DEV).manual_seed(0)
+
+    def parts():
+        total = sum(r * c for r, c in shapes) + 8 * (len(shapes) + 1)
+        buffer, at, views = torch.full((total,), float("nan"), device=DEV), 1, []
+        for k, (r, c) in enumerate(shapes):
+            views.append(buffer[at:at + r * c].view(r, c))
+            at += r * c + 2 * k + 1  # (odd gaps)
+        return buffer, views
+
+    values = [[torch.randn(s, device=DEV, generator=gen) for s in shapes] for _ in range(3)]
+    own = [torch.nn.Parameter(v.clone()) for v in values[0]]
+    buffers, placed = zip(*(parts() for _ in range(3)))
+    for views, vals in zip(placed, values):
+        for view, val in zip(views, vals):
+            view.copy_(val)
+    between = [b.isnan() for b in buffers]
+    apart = [torch.nn.Parameter(v) for v in placed[0]]
+    opts = optim.Muon(own, lr=0.02), optim.Muon(apart, lr=0.02)
+    for i, (p, q) in enumerate(zip(own, apart)):
+        assert q.data_ptr() == placed[0][i].data_ptr()
+        p.grad, q.grad = values[1][i], placed[1][i]
+        opts[0].state[p]["momentum_buffer"].copy_(values[2][i])
+        opts[1].state[q]["momentum_buffer"] = placed[2][i]
+    for _ in range(2):
+        for opt in opts:
+            opt.step()
+    for i, (p, q) in enumerate(zip(own, apart)):
+        assert torch.equal(p, q) and torch.equal(opts[0].state[p]["momentum_buffer"], placed[2][i])
+    assert all(torch.equal(b.isnan(), n) for b, n in zip(buffers, between))
