@@ -9,11 +9,11 @@
 // two planes take the bytes of one fp32 matrix.  The iteration bounds its own
 // entries -- |X_ij| <= |X|_2 <= u_t, with u_0 = |G|_F / (|G|_F + eps) and u_{t+1} the maximum of |a x + b x^3 + c x^5| on [0, u_t] --
 // so ONE scale per matrix and step is known before a product runs: no row maxima, and no fp16 overflow for any input.
-// What that gives up: planes hold a value to 2^-23 of itself (fp32: 2^-24) only down to 2^-16 u_t, where l becomes subnormal, and to 2^-37 u_t
-// below.  Sums of hundreds of fp32 terms lose more than 2^-23 of the norm, so in the norm the result is an fp32 iteration's (4096 x 4096: 3.0e-6 of
-// the 64-bit one, the library's fp32 products 4.6e-6); rows far weaker than the rest are not (200 x 400 graded 1 to 1e-6: the weakest are 2.5e-4 of
-// themselves off, 1e-5 with fp32 products; graded 1 to 1e-3 2e-6 and 9e-6).  An exponent per row would have to scale the contraction index of A and B X, whose operands are the same
-// planes.  An optimizer's direction asks for the norm.
+// What that gives up: planes hold a value to 2^-23 of itself (fp32: 2^-24) only down to 2^-16 u_t, where l becomes subnormal, and to 2^-37
+// u_t below.  Sums of hundreds of fp32 terms lose more than 2^-23 of the norm, so in the norm the result is an fp32 iteration's (4096 x 4096:
+// 3.0e-6 of the 64-bit one, the library's fp32 products 4.6e-6).  Rows far weaker than the rest are not (200 x 400 graded 1 to 1e-6: the weakest
+// are 2.5e-4 of themselves off, 1e-5 with fp32 products; graded 1 to 1e-3: 2e-6 and 9e-6).  An exponent per row would have to scale the
+// contraction index of A and B X, whose operands are the same planes; an optimizer's direction asks for the norm.
 // X is kept as X^T only: the product B X contracts along rows of B and of X^T (the fragments of an MFMA are 16-byte pieces of rows),
 // and X X^T contracts down the rows of X^T, whose fragments ds_read_b64_tr_b16 turns on their way out of LDS (keeping X as well
 // doubled what the last product writes and reads: ten 300 x 600 14.0 instead of 12.5 us).  A and B are symmetric: only the tiles on

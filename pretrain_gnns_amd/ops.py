@@ -1986,7 +1986,8 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     fp32, bf16 or fp16, or a list of such matrices of any sizes (one type and device): all of them share the launches.  Returns new
     contiguous tensors of the same type, rounded once; the same call gives the same bits.  Whatever the type, the result is as near as an
     iteration on fp32 products in the norm (Frobenius, spectral); rows (or columns) that are below 2^-16 of the others' size come out with
-    fewer than 22 bits of their own (1e-6: to some 3e-4 of themselves, fp32 products to 1e-5).  No gradient flows through it (it makes updates, not activations); a forward-mode tangent is refused."""
+    fewer than 22 bits of their own (1e-6: to some 3e-4 of themselves, fp32 products to 1e-5).  No gradient flows through it (it makes
+    updates, not activations); a forward-mode tangent and traces are refused."""
     import ctypes
     several = isinstance(g, (list, tuple))
     tensors = list(g) if several else [g]

@@ -169,9 +169,10 @@ class Muon:
     Per matrix  M <- momentum M + G;  U = G + momentum M (nesterov) or M;  O = ops.newton_schulz(U, ns_steps, ns_coefficients, eps);
     p <- p (1 - lr weight_decay) - lr s O  with s = sqrt(max(1, rows / cols)) (``adjust_lr_fn`` None or "original") or
     0.2 sqrt(max(rows, cols)) ("match_rms_adamw": updates as large as Adam's).  The arguments are those of torch.optim.Muon, and so is the
-    step but for three things.  The direction carries fp32's error (in the norm: ops.newton_schulz) where that class multiplies in bf16.  ``eps`` is added to the norm where that
-    class takes the larger of the two.  M is a sum where that class keeps an average (this M times 1 - momentum), which is the same direction
-    U / |U| but reaches eps at gradients 1 / (1 - momentum) times smaller: both matter for norms near eps only.
+    step but for three things.  The direction carries fp32's error (in the norm: ops.newton_schulz) where that class multiplies in bf16.
+    ``eps`` is added to the norm where that class takes the larger of the two.  M is a sum where that class keeps an average (this M times
+    1 - momentum), which is the same direction U / |U| but reaches eps at gradients 1 / (1 - momentum) times smaller: both matter for norms
+    near eps only.
 
     It takes 2-D parameters only (contiguous fp32 on one GPU): biases, norms' gains and embedding tables belong to ``Adam``.  The
     reference's loop body takes both in its optimizer list::
@@ -181,8 +182,8 @@ class Muon:
         optimizer_list = [Muon(weights, lr=0.02), Adam(others, lr=args.lr)]
 
     ``state[p]["momentum_buffer"]`` is p's M (zero before the first step).  A parameter without a gradient is skipped, momentum and
-    all.  lr, momentum, nesterov and weight_decay are read from ``param_groups[0]`` at every step; a captured step keeps the captured ones.  ns_steps, ns_coefficients, eps and
-    adjust_lr_fn are fixed when it is made.
+    all.  lr, momentum, nesterov and weight_decay are read from ``param_groups[0]`` at every step; a captured step keeps the captured ones.
+    ns_steps, ns_coefficients, eps and adjust_lr_fn are fixed when it is made.
     """
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7,
